@@ -39,6 +39,41 @@ def contiguous_bf16(t: torch.Tensor, name: str) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+# Element types as the kernels name them (ElemType in csrc/elementwise.cuh).
+ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def require_elem(t: torch.Tensor, name: str, allowed=tuple(ELEM)) -> None:
+    require(t.dtype in allowed, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in allowed)} (got {t.dtype})")
+
+
+def require_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        require(t is None or t.device == device, f"{name} must be on {device} (got {t.device if t is not None else None})")
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one: a kernel can only be launched there, and on its streams."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def rows_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as [rows, last dim] with unit stride along a row; a copy only where no such view exists."""
+    v = t.reshape(-1, t.shape[-1])
+    return v if v.shape[-1] == 1 or v.stride(-1) == 1 else v.contiguous()
+
+
 _declared = set()
 
 

@@ -240,3 +240,18 @@ def compare_with_dense(y: torch.Tensor, x: torch.Tensor, w_router: torch.Tensor,
     return dict(max_rel_err=err_clear, max_rel_err_all_tokens=err_all, ambiguous_tokens=int((~clear).sum()),
                 tokens=int(x.shape[0]), routing_ok=routing_ok, tol=tol,
                 ok=bool(routing_ok and err_clear <= tol))
+
+
+def rms_norm_ref(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float) -> torch.Tensor:
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension, in fp32 (fp64 inputs stay fp64)."""
+    x = x if x.dtype == torch.float64 else x.float()
+    y = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+    return y if weight is None else y * weight.to(x.dtype)
+
+
+def post_norm_ref(y: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], gate: Optional[torch.Tensor],
+                  norm: bool, residual_scale: float, next_weight: Optional[torch.Tensor], eps: float):
+    """(h, n or None): h = residual_scale * residual + gate * norm(y), n = norm(h), both unrounded."""
+    u = rms_norm_ref(y, weight, eps) if norm else (y if y.dtype == torch.float64 else y.float())
+    h = residual_scale * residual.to(u.dtype) + (u if gate is None else gate.to(u.dtype) * u)
+    return h, None if next_weight is None else rms_norm_ref(h, next_weight, eps)
