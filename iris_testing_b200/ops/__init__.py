@@ -3,6 +3,7 @@ kernels; CPU tensors run the PyTorch restatements in :mod:`.cpu_ref`."""
 from . import cpu_ref
 from ._common import check_default_status, default_status
 from .activation import silu_gate
+from .balance import balance_loss
 from .combine import padded_return, weighted_gather
 from .dispatch import AllToAllOp, custom_a2a, zero_padding
 from .expert import Expert, expert, grouped_gemm, to_kmajor

@@ -100,6 +100,15 @@ def default_status(device) -> torch.Tensor:
     return t
 
 
+def launch_status(device) -> torch.Tensor:
+    """:func:`default_status` for a launch that may be under capture into a graph.  The word itself cannot be made there: it
+    would live in that graph's memory and be zeroed by every replay."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _DEFAULT_STATUS and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("first call on this device is under graph capture: call the op, or default_status(device), once before")
+    return default_status(device)
+
+
 def check_default_status(device=None, reset: bool = True) -> None:
     """Raise if a kernel that was launched without a caller-owned status tensor has reported
     an error on ``device`` (default: the current device).  Synchronises."""

@@ -255,3 +255,30 @@ def post_norm_ref(y: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
     u = rms_norm_ref(y, weight, eps) if norm else (y if y.dtype == torch.float64 else y.float())
     h = residual_scale * residual.to(u.dtype) + (u if gate is None else gate.to(u.dtype) * u)
     return h, None if next_weight is None else rms_norm_ref(h, next_weight, eps)
+
+
+def balance_loss_ref(logits: torch.Tensor, topk_idx: torch.Tensor, balance_coef: float, z_coef: float,
+                     seq_rows: Optional[torch.Tensor], token_mask: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss, counts int32 [S, E]) with the semantics of ``ops.balance_loss``; fp32 (fp64 logits stay fp64)."""
+    T, E = logits.shape
+    k = topk_idx.shape[1]
+    lg = logits if logits.dtype == torch.float64 else logits.float()
+    top = lg.detach().amax(1) if T else lg.detach().sum(1)
+    part = torch.isfinite(top) & (top > torch.finfo(logits.dtype).min)
+    if token_mask is not None:
+        part = part & token_mask
+    lengths = [T] if seq_rows is None else seq_rows.clamp(min=0).tolist()
+    S = len(lengths)
+    seq = torch.repeat_interleave(torch.arange(S), torch.tensor(lengths, dtype=torch.int64))[:T]
+    seq = torch.cat((seq, torch.full((T - seq.numel(),), S)))
+    part = part & (seq < S)
+    t = part.nonzero().squeeze(1)
+    seq, lg, idx = seq[t], lg[t], topk_idx[t].long()
+    hit = (idx >= 0) & (idx < E)
+    counts = torch.bincount((seq.unsqueeze(1) * E + idx)[hit], minlength=S * E).view(S, E)
+    n_s = torch.bincount(seq, minlength=S).to(lg.dtype)
+    prob = torch.zeros(S, E, dtype=lg.dtype).index_add(0, seq, torch.softmax(lg, 1))
+    some = n_s.clamp(min=1.0)
+    terms = E * (counts.to(lg.dtype) * prob).sum(1) / (k * some * some)
+    z = torch.logsumexp(lg, 1).pow(2).sum() / max(t.numel(), 1)
+    return balance_coef * terms.sum() / max(int((n_s > 0).sum()), 1) + z_coef * z, counts.to(torch.int32)
