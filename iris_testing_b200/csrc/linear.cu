@@ -1,0 +1,806 @@
+// Matrix products with bias, activation and residual in their epilogue, dense or with one weight per group of packed
+// rows, and their backward products, on tcgen05 tensor cores.
+//
+//   forward   z_g = x_g W_g^T + b_g,  y = act(z) + res          x [M, K], W [G, N, K]
+//   dX        dx_g = dz_g W_g                                    dz = dy act'(z), [M, N]
+//   dW        dW_g = dz_g^T x_g                                  db_g = column sums of dz_g
+//
+// One persistent kernel for the three products: warp 0 loads (TMA), warp 1 issues the MMAs, warps 2-5 drain the
+// accumulators, warps 6-7 mend ragged ends.  An operand whose contracted dimension is contiguous is K-major
+// (x and W forward, dz for dX); the others (W for dX, both of dW) are read as they lie in memory, MN-major, in boxes of 64
+// columns x 64 contracted rows, so that nothing is ever transposed in memory.
+//
+// dW contracts over a group's rows, whose end lies anywhere inside a block of 64.  The rows of the last block that
+// belong to the next group (or to nothing) are set to zero in shared memory, in both operands, so that what lies there,
+// infinities and NaN included, has no part in the product.
+//
+// The hidden pre-activations z are kept for the backward pass in the element type; dz is rounded to it too, since the
+// tensor cores multiply 16-bit values: two roundings of half a step each that average out over the contracted dimension.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <atomic>
+
+#include "elementwise.cuh"
+#include "launch.h"
+#include "moe_args.h"
+#include "sm100_ptx.cuh"
+#include "tile_order.cuh"
+
+extern "C" {
+typedef struct b200_linear_args {
+  const void* a;            // forward: x [M, K]; dX: dz [M, N]; dW: dz [M, N]
+  const void* b;            // forward, dX: W [G, N, K]; dW: x [M, K]
+  void* out;                // y [M, n_out]; dx [M, K]; dW [G, N, K]
+  void* z;                  // forward: [M, N] or null
+  const void* bias;         // [G, N] or null
+  const void* res;          // [M, n_out] or null
+  const int* group_rows;    // [G] or null: one group of all M rows
+  int* status;
+  unsigned long long wait_budget_ns;
+  int mode;                 // LinearMode
+  int G, M, N, K, n_out;
+  int elem;                 // ELEM_BF16 or ELEM_F16
+  int act;                  // LinearAct
+  int pair;                 // two CTAs per tile (256 rows)
+  int group_m;              // M-tiles per chunk (see decode_tile)
+} b200_linear_args;
+
+typedef struct b200_act_grad_args {
+  const void* dy;           // [M, n_out]
+  const void* z;            // [M, N] or null (no activation)
+  void* dz;                 // [M, N] or null (no activation: dz is dy)
+  void* dres;               // [M, n_out] or null: dy of the groups' rows, zero behind them
+  void* dbias;              // [G, N] or null
+  float* record;            // [chunks + G][N] sums over the rows of a group in a chunk
+  const int* group_rows;
+  int G, M, N, n_out, elem, act;
+  int chunks, chunk_rows;
+} b200_act_grad_args;
+}
+
+namespace b200 {
+
+enum LinearMode : int { LIN_FORWARD = 0, LIN_DX = 1, LIN_DW = 2 };
+enum LinearAct : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SILU_GATE = 4 };
+
+constexpr int LBM = 128;                 // rows of a tile per CTA
+constexpr int LBN = 256;                 // columns of a tile
+constexpr int LBK = 64;                  // contracted elements per stage
+constexpr int LIN_THREADS = 256;
+constexpr int LIN_MENDERS = 2;           // warps 6 and 7
+constexpr int LIN_A_BYTES = LBM * LBK * 2;
+constexpr int LIN_MN_BOX = 64 * LBK * 2; // bytes of one MN-major box
+constexpr int LIN_BOX = 32 * 128;        // a warp's staging box: 32 rows x 64 columns, 16-byte chunks XOR-swizzled by row
+
+// Stages and staging boxes per variant.  Forward: three boxes per epilogue warp (z of the gate, z of the up half, y);
+// the products without z need one.
+template <int MODE, int CG>
+struct LinGeo {
+  static constexpr int B_ROWS = LBN / CG;
+  static constexpr int B_BYTES = B_ROWS * LBK * 2;
+  static constexpr int STAGE = LIN_A_BYTES + B_BYTES;
+  static constexpr int BOXES = MODE == LIN_FORWARD ? 3 : 1;
+  static constexpr int STAGES = CG == 2 ? (MODE == LIN_FORWARD ? 5 : 6) : (MODE == LIN_FORWARD ? 3 : 4);
+  static constexpr int TM = LBM * CG;
+};
+constexpr int LIN_MAX_STAGES = 6;
+
+struct __align__(16) LinControl {
+  uint64_t full[LIN_MAX_STAGES], empty[LIN_MAX_STAGES];
+  uint64_t part_full[LIN_MAX_STAGES];    // dW: this CTA's own bytes of a block that has to be mended
+  uint64_t mended[LIN_MAX_STAGES];       // dW: both CTAs have mended theirs
+  uint64_t tmem_full[2], tmem_empty[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int g_rows[B200_MAX_GROUPS];
+  int g_row_start[B200_MAX_GROUPS + 1];
+  int g_sched_start[B200_MAX_GROUPS + 1];
+};
+template <int MODE, int CG>
+constexpr int lin_smem() {
+  using S = LinGeo<MODE, CG>;
+  return S::STAGES * S::STAGE + 4 * S::BOXES * LIN_BOX + static_cast<int>(sizeof(LinControl)) + 1024;
+}
+static_assert(lin_smem<LIN_FORWARD, 1>() <= 232448 && lin_smem<LIN_FORWARD, 2>() <= 232448 && lin_smem<LIN_DW, 1>() <= 232448 &&
+                  lin_smem<LIN_DW, 2>() <= 232448, "exceeds 227 KiB of shared memory per CTA");
+
+// 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
+__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+constexpr float GELU_A = 0.7978845608028654f, GELU_B = 0.044715f;    // tanh form: v * sigmoid(2 A (v + B v^3))
+__device__ __forceinline__ float act_value(float v, int act) {
+  if (act == ACT_RELU) return v < 0.f ? 0.f : v;
+  if (act == ACT_SILU) return v * sigmoid_f(v);
+  if (act == ACT_GELU) return v * sigmoid_f(2.f * GELU_A * (v + GELU_B * v * v * v));
+  return v;
+}
+__device__ __forceinline__ float act_slope(float v, int act) {
+  if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
+  if (act == ACT_SILU) {
+    const float q = sigmoid_f(v);
+    return q * (1.f + v * (1.f - q));
+  }
+  if (act == ACT_GELU) {
+    const float q = sigmoid_f(2.f * GELU_A * (v + GELU_B * v * v * v));
+    return q + v * q * (1.f - q) * 2.f * GELU_A * (1.f + 3.f * GELU_B * v * v);
+  }
+  return 1.f;
+}
+
+__device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
+  if (bf16) return pack_bf16x2(lo, hi);
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_16(uint32_t v, bool bf16) {
+  if (bf16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// Rows and first row of every group, and its first scheduling tile (tiles per group: by its rows, or `fixed`).  One warp.
+// Returns the rows of all groups.
+__device__ __forceinline__ long long lin_scan(LinControl& c, const int* group_rows, int G, int M, int lane, int tile_rows, int fixed) {
+  long long carry = 0;
+  int tcarry = 0;
+  for (int base = 0; base < G; base += 32) {
+    const int g = base + lane;
+    const int rows = g < G ? (group_rows != nullptr ? max(0, group_rows[g]) : M) : 0;
+    const int tiles = g < G ? (fixed > 0 ? fixed : (rows + tile_rows - 1) / tile_rows) : 0;
+    long long rs = rows;
+    int ts = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long r2 = __shfl_up_sync(0xffffffffu, rs, o);
+      const int t2 = __shfl_up_sync(0xffffffffu, ts, o);
+      if (lane >= o) { rs += r2; ts += t2; }
+    }
+    if (g < G) {
+      c.g_rows[g] = rows;
+      c.g_row_start[g] = static_cast<int>(min(carry + rs - rows, 0x7fffffffll));
+      c.g_sched_start[g] = tcarry + ts - tiles;
+    }
+    carry += __shfl_sync(0xffffffffu, rs, 31);
+    tcarry += __shfl_sync(0xffffffffu, ts, 31);
+  }
+  if (lane == 0) {
+    c.g_row_start[G] = static_cast<int>(min(carry, 0x7fffffffll));
+    c.g_sched_start[G] = tcarry;
+  }
+  return carry;
+}
+
+// Writes one staging box: 32 rows x 64 columns at (row, col) of a row-major matrix.  Whole boxes leave as one bulk tensor
+// store, others row segment by row segment.
+__device__ __forceinline__ void store_box(uint8_t* box, const CUtensorMap* tmap, char* base, long long ld_bytes, long long row,
+                                          int col, int cols, int rows_here, int lane, bool& pending) {
+  if (rows_here >= 32) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && col < cols) {
+      tma_store_2d(tmap, box, col, static_cast<int>(row));
+      bulk_commit_group();
+      pending = true;
+    }
+    return;
+  }
+  __syncwarp();
+  const int c = col + (lane & 7) * 8;
+#pragma unroll
+  for (int rr = 0; rr < 8; ++rr) {
+    const int r = rr * 4 + (lane >> 3);
+    if (r < rows_here && c < cols)
+      st_16(base + (row + r) * ld_bytes + c * 2ll, *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4)));
+  }
+  __syncwarp();
+}
+
+template <int MODE, int CG, bool GATED>
+__global__ void __launch_bounds__(LIN_THREADS, 1)
+linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+              const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_z, const b200_linear_args la) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  using S = LinGeo<MODE, CG>;
+  constexpr int STAGES = S::STAGES;
+  constexpr bool A_MN = MODE == LIN_DW, B_MN = MODE != LIN_FORWARD;
+  uint8_t* staging = smem + STAGES * S::STAGE;
+  LinControl& c = *reinterpret_cast<LinControl*>(staging + 4 * S::BOXES * LIN_BOX);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = la.G;
+  const uint32_t cta_rank = CG == 2 ? cluster_ctarank() : 0u;
+  const bool bf16 = la.elem == ELEM_BF16;
+  // the product's own sizes: rows of a tile's group (dW: features), columns, contracted length of a group
+  const int cols = MODE == LIN_FORWARD ? la.N : la.K;
+  const int TN = (cols + LBN - 1) / LBN;
+
+  WaitCtx w;
+  w.abort_flag = &c.abort_flag;
+  w.status = la.status;
+  w.budget_ns = la.wait_budget_ns;
+
+  if (tid == 0) {
+    c.abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&c.full[s], 1);
+      mbar_init(&c.empty[s], 1);
+      mbar_init(&c.part_full[s], 1);
+      mbar_init(&c.mended[s], LIN_MENDERS * CG);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&c.tmem_full[a], 1);
+      mbar_init(&c.tmem_empty[a], 128 * CG);
+    }
+    mbar_init(&c.drain, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_o);
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(&c.tmem_base, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&c.tmem_base, 512);
+      tmem_relinquish();
+    }
+  }
+  __syncthreads();                      // abort_flag is set below
+  if (warp == 0) {
+    const long long rows = lin_scan(c, la.group_rows, G, la.M, lane, S::TM, MODE == LIN_DW ? (la.N + S::TM - 1) / S::TM : 0);
+    // more rows than the buffers hold: nothing is computed, the host reads the status
+    if (lane == 0 && rows > la.M) {
+      report_status(w.status, ST_OVERFLOW);
+      if (w.status != nullptr) atomicMax(w.status + 1, c.g_row_start[G]);
+      c.abort_flag = 1;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();      // the peer's barriers exist before anyone signals them
+  tc_fence_after_sync();
+
+  const uint32_t tmem_base = c.tmem_base;
+  const bool overflow = c.abort_flag != 0;
+  const int total_tiles = overflow ? 0 : c.g_sched_start[G] * TN;
+  int tile_first, tile_stride;
+  tile_walk(total_tiles, gridDim.x / CG, blockIdx.x / CG, tile_first, tile_stride);
+  // every role reads the flag above before any of them may set it
+  __syncthreads();
+
+  // blocks of the contracted dimension in a tile of group g
+  auto k_blocks = [&](int g) { return ((MODE == LIN_FORWARD ? la.K : MODE == LIN_DX ? la.N : c.g_rows[g]) + LBK - 1) / LBK; };
+  // dW: contracted rows in the last block of group g (64: whole)
+  auto tail_rows = [&](int g) { return MODE == LIN_DW ? ((c.g_rows[g] - 1) & (LBK - 1)) + 1 : LBK; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      int cursor = 0, stage = 0, issued = 0;
+      uint32_t phase = 0, part_phase = 0, part_used = 0;      // a bit per stage
+      bool ok = true;
+      for (int idx = tile_first; ok && idx < total_tiles; idx += tile_stride) {
+        int g, m, n;
+        if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
+        const int KB = k_blocks(g);
+        const bool ragged = tail_rows(g) < LBK;
+        const int mrow = m * S::TM + static_cast<int>(cta_rank) * LBM;      // first row (dW: feature) of my half
+        const int ncol = n * LBN + static_cast<int>(cta_rank) * S::B_ROWS;  // first column of my share of B
+        const int row0 = c.g_row_start[g];
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!mbar_wait(&c.empty[stage], phase ^ 1u, w, ST_TIMEOUT_PIPE_EMPTY)) { ok = false; break; }
+          uint8_t* sa = smem + stage * S::STAGE;
+          uint8_t* sb = sa + LIN_A_BYTES;
+          const bool part = MODE == LIN_DW && ragged && kb == KB - 1;
+          if (part) {
+            // this CTA's bytes go to its own barrier; the pair's goes on at once, the MMAs wait for `mended`
+            if (cta_rank == 0) mbar_arrive(&c.full[stage]);
+            mbar_expect_tx(&c.part_full[stage], S::STAGE);
+#pragma unroll
+            for (int i = 0; i < LBM / 64; ++i)
+              tma_load_2d(sa + i * LIN_MN_BOX, &tmap_a, &c.part_full[stage], mrow + i * 64, row0 + kb * LBK);
+#pragma unroll
+            for (int i = 0; i < S::B_ROWS / 64; ++i)
+              tma_load_2d(sb + i * LIN_MN_BOX, &tmap_b, &c.part_full[stage], ncol + i * 64, row0 + kb * LBK);
+            part_phase ^= 1u << stage;
+            part_used |= 1u << stage;
+          } else if constexpr (CG == 2) {
+            if (cta_rank == 0) mbar_expect_tx(&c.full[stage], S::STAGE * 2);
+            const uint32_t bar = map_to_cta(&c.full[stage], 0);
+            if constexpr (A_MN) {
+#pragma unroll
+              for (int i = 0; i < LBM / 64; ++i) tma_load_2d_pair(sa + i * LIN_MN_BOX, &tmap_a, bar, mrow + i * 64, row0 + kb * LBK);
+            } else {
+              tma_load_2d_pair(sa, &tmap_a, bar, kb * LBK, row0 + mrow);
+            }
+            if constexpr (MODE == LIN_FORWARD) {
+              tma_load_2d_pair(sb, &tmap_b, bar, kb * LBK, g * la.N + ncol);
+            } else {
+#pragma unroll
+              for (int i = 0; i < S::B_ROWS / 64; ++i) {
+                if constexpr (MODE == LIN_DX) tma_load_3d_pair(sb + i * LIN_MN_BOX, &tmap_b, bar, ncol + i * 64, kb * LBK, g);
+                else tma_load_2d_pair(sb + i * LIN_MN_BOX, &tmap_b, bar, ncol + i * 64, row0 + kb * LBK);
+              }
+            }
+          } else {
+            mbar_expect_tx(&c.full[stage], S::STAGE);
+            if constexpr (A_MN) {
+#pragma unroll
+              for (int i = 0; i < LBM / 64; ++i) tma_load_2d(sa + i * LIN_MN_BOX, &tmap_a, &c.full[stage], mrow + i * 64, row0 + kb * LBK);
+            } else {
+              tma_load_2d(sa, &tmap_a, &c.full[stage], kb * LBK, row0 + mrow);
+            }
+            if constexpr (MODE == LIN_FORWARD) {
+              tma_load_2d(sb, &tmap_b, &c.full[stage], kb * LBK, g * la.N + ncol);
+            } else {
+#pragma unroll
+              for (int i = 0; i < S::B_ROWS / 64; ++i) {
+                if constexpr (MODE == LIN_DX) tma_load_3d(sb + i * LIN_MN_BOX, &tmap_b, &c.full[stage], ncol + i * 64, kb * LBK, g);
+                else tma_load_2d(sb + i * LIN_MN_BOX, &tmap_b, &c.full[stage], ncol + i * 64, row0 + kb * LBK);
+              }
+            }
+          }
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // Retire the loads still in flight before shared memory is released.  The pair leader's barriers account for both
+      // CTAs' loads; blocks to be mended are on each CTA's own.
+      int no_abort = 0;
+      WaitCtx wd = w;
+      wd.abort_flag = &no_abort;
+      const int behind = CG == 2 && cta_rank != 0 ? 0 : min(issued, STAGES);
+      for (int i = 0; i < behind; ++i) {
+        int s = stage - 1 - i;
+        uint32_t ph = phase;
+        if (s < 0) { s += STAGES; ph ^= 1u; }
+        mbar_wait(&c.full[s], ph, wd, ST_TIMEOUT_DRAIN);
+      }
+      for (int s = 0; s < STAGES; ++s)
+        if (part_used >> s & 1u) mbar_wait(&c.part_full[s], (part_phase >> s & 1u) ^ 1u, wd, ST_TIMEOUT_DRAIN);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs
+    if (lane == 0 && cta_rank == 0) {
+      const uint32_t idesc = make_idesc_16bit(S::TM, LBN, bf16, A_MN, B_MN);
+      int cursor = 0, stage = 0, it = 0;
+      uint32_t phase = 0, mend_phase = 0;
+      bool ok = true;
+      for (int idx = tile_first; ok && idx < total_tiles; idx += tile_stride, ++it) {
+        int g, m, n;
+        if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
+        const int KB = k_blocks(g);
+        const bool ragged = tail_rows(g) < LBK;
+        const int acc = it & 1;
+        if (!mbar_wait(&c.tmem_empty[acc], ((it >> 1) & 1) ^ 1u, w, ST_TIMEOUT_TMEM_EMPTY)) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + acc * LBN;
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!mbar_wait(&c.full[stage], phase, w, ST_TIMEOUT_PIPE_FULL)) { ok = false; break; }
+          if (MODE == LIN_DW && ragged && kb == KB - 1) {
+            if (!mbar_wait_cluster(&c.mended[stage], mend_phase >> stage & 1u, w, ST_TIMEOUT_PIPE_FULL)) { ok = false; break; }
+            mend_phase ^= 1u << stage;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * S::STAGE), sb = sa + LIN_A_BYTES;
+          const uint64_t ad = A_MN ? make_smem_desc_mn_sw128(sa, LIN_MN_BOX) : make_smem_desc_sw128(sa);
+          const uint64_t bd = B_MN ? make_smem_desc_mn_sw128(sb, LIN_MN_BOX) : make_smem_desc_sw128(sb);
+          // 16 steps of K: 32 bytes along a K-major row, 2048 bytes down an MN-major box
+          constexpr int ASTEP = A_MN ? 2048 / 16 : 2, BSTEP = B_MN ? 2048 / 16 : 2;
+#pragma unroll
+          for (int k = 0; k < LBK / 16; ++k) {
+            if constexpr (CG == 2) umma_bf16_ss_pair(d, ad + ASTEP * k, bd + BSTEP * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            else umma_bf16_ss(d, ad + ASTEP * k, bd + BSTEP * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          if constexpr (CG == 2) umma_commit_pair(&c.empty[stage], 3);
+          else umma_commit(&c.empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if constexpr (CG == 2) umma_commit_pair(&c.tmem_full[acc], 3);
+        else umma_commit(&c.tmem_full[acc]);
+      }
+      if constexpr (CG == 2) umma_commit_pair(&c.drain, 1);
+      else umma_commit(&c.drain);
+      int no_abort = 0;
+      WaitCtx wd = w;
+      wd.abort_flag = &no_abort;
+      mbar_wait(&c.drain, 0, wd, ST_TIMEOUT_DRAIN);
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ epilogue
+    constexpr int OUT_TILE = GATED ? LBN / 2 : LBN;
+    const int q = warp & 3;                            // TMEM lane quarter this warp may read
+    uint8_t* boxes = staging + q * S::BOXES * LIN_BOX;
+    uint8_t* ybox = boxes;
+    uint8_t* zbox = boxes + LIN_BOX;                   // forward: z, or the gate's z with the up half's behind it
+    bool pending = false;                              // lane 0: a bulk store may still be reading a box
+    int cursor = 0, it = 0;
+    const uint32_t empty_addr[2] = {map_to_cta(&c.tmem_empty[0], 0), map_to_cta(&c.tmem_empty[1], 0)};
+    for (int idx = tile_first; idx < total_tiles; idx += tile_stride, ++it) {
+      int g, m, n;
+      if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
+      const int acc = it & 1;
+      const int half0 = m * S::TM + static_cast<int>(cta_rank) * LBM + q * 32;     // this warp's first row in the group
+      const int rows_here = (MODE == LIN_DW ? la.N : c.g_rows[g]) - half0;         // may be <= 0
+      const long long row0 = MODE == LIN_DW ? static_cast<long long>(g) * la.N + half0 : c.g_row_start[g] + half0;
+      const bool zero = MODE == LIN_DW && c.g_rows[g] == 0;
+      const bool got = mbar_wait(&c.tmem_full[acc], (it >> 1) & 1, w, ST_TIMEOUT_TMEM_FULL);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after_sync();
+      const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * LBN;
+      const bool row_ok = lane < rows_here;
+#pragma unroll 1
+      for (int p = 0; p < OUT_TILE / 64; ++p) {
+        const int ycol = n * OUT_TILE + p * 64;        // first output column of the pass
+        if (pending) bulk_wait_group_read<0>();        // lane 0: the last pass's stores have read the boxes
+        pending = false;
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int cc = p * 64 + h * 32;
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_acc + cc, v);
+          uint32_t u[GATED ? 32 : 1];
+          if constexpr (GATED) tmem_ld_32x32b_x32(t_acc + LBN / 2 + cc, u);
+          tmem_ld_wait();
+          if (zero) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0u;
+          }
+          if constexpr (MODE == LIN_FORWARD) {
+            const int zcol = n * LBN + cc;             // column of z (of the gate half)
+            auto add_bias = [&](uint32_t (&x)[32], int col) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (col + i * 8 >= la.N) continue;
+                const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const char*>(la.bias) + (static_cast<size_t>(g) * la.N + col + i * 8) * 2);
+                const uint32_t bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float2 f = unpack_16(bb[j], bf16);
+                  x[i * 8 + 2 * j] = __float_as_uint(__uint_as_float(x[i * 8 + 2 * j]) + f.x);
+                  x[i * 8 + 2 * j + 1] = __float_as_uint(__uint_as_float(x[i * 8 + 2 * j + 1]) + f.y);
+                }
+              }
+            };
+            if (la.bias != nullptr) {
+              add_bias(v, zcol);
+              if constexpr (GATED) add_bias(reinterpret_cast<uint32_t(&)[32]>(u), zcol + LBN / 2);
+            }
+            if (la.z != nullptr) {
+              auto put = [&](const uint32_t (&x)[32], uint8_t* box) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
+                      make_uint4(pack_16(__uint_as_float(x[8 * i]), __uint_as_float(x[8 * i + 1]), bf16),
+                                 pack_16(__uint_as_float(x[8 * i + 2]), __uint_as_float(x[8 * i + 3]), bf16),
+                                 pack_16(__uint_as_float(x[8 * i + 4]), __uint_as_float(x[8 * i + 5]), bf16),
+                                 pack_16(__uint_as_float(x[8 * i + 6]), __uint_as_float(x[8 * i + 7]), bf16));
+              };
+              put(v, zbox);
+              if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), zbox + LIN_BOX);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float f = __uint_as_float(v[i]);
+              if constexpr (GATED) v[i] = __float_as_uint(f * sigmoid_f(f) * __uint_as_float(u[i]));
+              else v[i] = __float_as_uint(act_value(f, la.act));
+            }
+            if (la.res != nullptr && row_ok) {
+              const int col = ycol + h * 32;
+              const char* src = static_cast<const char*>(la.res) + ((row0 + lane) * la.n_out + col) * 2;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (col + i * 8 >= la.n_out) continue;
+                const uint4 b = ld_16(src + i * 16);
+                const uint32_t bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float2 f = unpack_16(bb[j], bf16);
+                  v[i * 8 + 2 * j] = __float_as_uint(__uint_as_float(v[i * 8 + 2 * j]) + f.x);
+                  v[i * 8 + 2 * j + 1] = __float_as_uint(__uint_as_float(v[i * 8 + 2 * j + 1]) + f.y);
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(ybox + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_16(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]), bf16),
+                           pack_16(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]), bf16),
+                           pack_16(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]), bf16),
+                           pack_16(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]), bf16));
+        }
+        if (p == OUT_TILE / 64 - 1) {
+          tc_fence_before_sync();
+          if constexpr (CG == 2) mbar_arrive_cluster(empty_addr[acc]);
+          else mbar_arrive(&c.tmem_empty[acc]);
+        }
+        store_box(ybox, &tmap_o, static_cast<char*>(la.out), static_cast<long long>(la.n_out) * 2, row0, ycol, la.n_out, rows_here, lane, pending);
+        if constexpr (MODE == LIN_FORWARD) {
+          if (la.z != nullptr) {
+            const long long ldz = static_cast<long long>(la.N) * 2;
+            store_box(zbox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + p * 64, la.N, rows_here, lane, pending);
+            if constexpr (GATED)
+              store_box(zbox + LIN_BOX, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + LBN / 2 + p * 64, la.N, rows_here, lane, pending);
+          }
+        }
+      }
+    }
+    if (pending) bulk_wait_group<0>();                 // shared memory stays allocated until the stores are done
+  } else {
+    // ------------------------------------------------------------ ragged ends
+    if constexpr (MODE == LIN_DW) {
+      int cursor = 0, blocks = 0;
+      uint32_t phase = 0;
+      for (int idx = tile_first; idx < total_tiles; idx += tile_stride) {
+        int g, m, n;
+        if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
+        const int KB = k_blocks(g);
+        blocks += KB;
+        const int tail = tail_rows(g);
+        if (KB == 0 || tail == LBK) continue;
+        const int stage = (blocks - 1) % STAGES;
+        const bool got = mbar_wait(&c.part_full[stage], phase >> stage & 1u, w, ST_TIMEOUT_PIPE_FULL);
+        if (!__all_sync(0xffffffffu, got)) break;
+        phase ^= 1u << stage;
+        uint8_t* s = smem + stage * S::STAGE;
+        constexpr int NBOX = S::STAGE / LIN_MN_BOX;
+        // rows [tail, 64) of every box: whole 128-byte rows, which the swizzle does not leave
+        for (int i = tid - 6 * 32; i < NBOX * (LBK - tail) * 8; i += LIN_MENDERS * 32) {
+          const int box = i / ((LBK - tail) * 8), r = i - box * (LBK - tail) * 8;
+          *reinterpret_cast<uint4*>(s + box * LIN_MN_BOX + tail * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_cluster(map_to_cta(&c.mended[stage], 0));
+          else mbar_arrive(&c.mended[stage]);
+        }
+      }
+    } else if (!overflow) {
+      // rows of the buffer behind the last group
+      const long long first = static_cast<long long>(c.g_row_start[G]) * la.n_out / 8, last = static_cast<long long>(la.M) * la.n_out / 8;
+      uint4* out = reinterpret_cast<uint4*>(la.out);
+      const long long step = static_cast<long long>(gridDim.x) * LIN_MENDERS * 32;
+      for (long long i = first + blockIdx.x * (LIN_MENDERS * 32) + tid - 6 * 32; i < last; i += step) out[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// dz = act'(z) dy and the column sums of dz over each group.  A block takes eight columns per thread of a run of rows;
+// the sums of a (run, group) go to record run + group (both only ever advance), added up in order by the next kernel.
+template <typename T>
+__global__ void __launch_bounds__(128) act_grad_kernel(const b200_act_grad_args a) {
+  const bool gated = a.act == ACT_SILU_GATE;
+  // a thread's eight columns of the output; of the gated form they belong to eight columns of the gate and of the up half
+  const int oc = (blockIdx.y * 128 + threadIdx.x) * 8;
+  const bool in = oc < a.n_out;
+  const int zc = gated ? (oc / 128) * 256 + oc % 128 : oc;
+  long long start = 0;
+  int g = 0;
+  const long long r0 = static_cast<long long>(blockIdx.x) * a.chunk_rows, r1 = min(static_cast<long long>(a.M), r0 + a.chunk_rows);
+  auto rows_of = [&](int i) { return a.group_rows != nullptr ? max(0, a.group_rows[i]) : a.M; };
+  while (g < a.G && start + rows_of(g) <= r0) start += rows_of(g++);
+  long long pos = r0;
+  for (; g < a.G && pos < r1; ++g) {
+    const long long end = min(r1, start + rows_of(g));
+    start += rows_of(g);
+    if (end <= pos) continue;
+    float sum[8], sum2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] = sum2[j] = 0.f;
+    if (in) {
+      for (long long r = pos; r < end; ++r) {
+        float d[8], z[8], u[8];
+        load_pack<T, 8>(static_cast<const T*>(a.dy) + r * a.n_out + oc, d);
+        if (a.dres != nullptr) store_pack<T, 8>(static_cast<T*>(a.dres) + r * a.n_out + oc, d);
+        if (a.z != nullptr) {
+          load_pack<T, 8>(static_cast<const T*>(a.z) + r * a.N + zc, z);
+          if (gated) {
+            load_pack<T, 8>(static_cast<const T*>(a.z) + r * a.N + zc + 128, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float q = sigmoid_f(z[j]);
+              const float du = d[j] * z[j] * q;
+              d[j] *= u[j] * q * (1.f + z[j] * (1.f - q));
+              u[j] = du;
+              sum2[j] += du;
+            }
+            store_pack<T, 8>(static_cast<T*>(a.dz) + r * a.N + zc + 128, u);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] *= act_slope(z[j], a.act);
+          }
+          store_pack<T, 8>(static_cast<T*>(a.dz) + r * a.N + zc, d);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += d[j];
+      }
+      if (a.dbias != nullptr) {
+        float* rec = a.record + (static_cast<size_t>(blockIdx.x) + g) * a.N;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          rec[zc + j] = sum[j];
+          if (gated) rec[zc + 128 + j] = sum2[j];
+        }
+      }
+    }
+    pos = end;
+  }
+  if (a.dres != nullptr && in) {
+    const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (long long r = pos; r < r1; ++r) store_pack<T, 8>(static_cast<T*>(a.dres) + r * a.n_out + oc, none);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) bias_grad_kernel(const b200_act_grad_args a) {
+  chain_wait();
+  const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  long long start = 0;
+  for (int i = 0; i < g; ++i) start += max(0, a.group_rows[i]);
+  const long long rows = a.group_rows != nullptr ? max(0, a.group_rows[g]) : a.M;
+  const long long end = min(static_cast<long long>(a.M), start + rows);
+  float v = 0.f;
+  if (c < a.N) {
+    if (end > start)
+      for (long long k = start / a.chunk_rows; k <= (end - 1) / a.chunk_rows; ++k) v += a.record[(static_cast<size_t>(k) + g) * a.N + c];
+    static_cast<T*>(a.dbias)[static_cast<size_t>(g) * a.N + c] = from_f32<T>(v);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+typedef CUresult (*LinEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static LinEncodeFn lin_encode() {
+  static std::atomic<void*> fn{nullptr};
+  void* p = fn.load(std::memory_order_relaxed);
+  if (p == nullptr) {
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess) return nullptr;
+    fn.store(p, std::memory_order_relaxed);
+  }
+  return reinterpret_cast<LinEncodeFn>(p);
+}
+
+// Row-major [planes][rows][cols] of 16-bit elements (two dimensions where planes is 0), boxes of 64 columns x box_rows.
+static int lin_map(CUtensorMap* tm, const void* base, int elem, long long planes, long long rows, long long cols, int box_rows) {
+  LinEncodeFn enc = lin_encode();
+  if (enc == nullptr) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || cols % 8 != 0 || rows <= 0) return -2;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * 2, static_cast<cuuint64_t>(cols) * rows * 2};
+  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_rows), 1u};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(tm, elem == ELEM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes > 0 ? 3 : 2,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
+// Sets a kernel's shared-memory limit once per device, and makes the device's context current: the thread that runs a
+// backward pass may not have met it yet, and tensor maps are encoded by the driver, which does not do so itself.
+template <typename K>
+static cudaError_t lin_configure(K kern, int smem, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1ull)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+
+template <int MODE, int CG, bool GATED>
+static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) {
+  static std::atomic<unsigned long long> configured{0};
+  using S = LinGeo<MODE, CG>;
+  auto kern = linear_kernel<MODE, CG, GATED>;
+  constexpr int smem = lin_smem<MODE, CG>();
+  const cudaError_t e = lin_configure(kern, smem, configured);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  CUtensorMap ta, tb, to, tz;
+  const long long out_rows = MODE == LIN_DW ? static_cast<long long>(la.G) * la.N : la.M;
+  int r = MODE == LIN_FORWARD ? lin_map(&ta, la.a, la.elem, 0, la.M, la.K, LBM)
+          : MODE == LIN_DX    ? lin_map(&ta, la.a, la.elem, 0, la.M, la.N, LBM)
+                              : lin_map(&ta, la.a, la.elem, 0, la.M, la.N, LBK);
+  if (r == 0)
+    r = MODE == LIN_FORWARD ? lin_map(&tb, la.b, la.elem, 0, static_cast<long long>(la.G) * la.N, la.K, S::B_ROWS)
+        : MODE == LIN_DX    ? lin_map(&tb, la.b, la.elem, la.G, la.N, la.K, LBK)
+                            : lin_map(&tb, la.b, la.elem, 0, la.M, la.K, LBK);
+  if (r == 0) r = lin_map(&to, la.out, la.elem, 0, out_rows, la.n_out, 32);
+  tz = to;
+  if (r == 0 && la.z != nullptr) r = lin_map(&tz, la.z, la.elem, 0, la.M, la.N, 32);
+  if (r != 0) return r;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(ctas / CG * CG, 1, 1);
+  cfg.blockDim = dim3(LIN_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  b200_count_launches(1);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tz, la));
+}
+
+}  // namespace b200
+
+extern "C" {
+
+int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
+  using namespace b200;
+  if (args == nullptr || args->G < 1 || args->G > B200_MAX_GROUPS || args->M < 1 || args->N < 1 || args->K < 1 || ctas < 2) return -10;
+  b200_linear_args la = *args;
+  if (la.N % 8 != 0 || la.K % 8 != 0 || (la.elem != ELEM_BF16 && la.elem != ELEM_F16)) return -11;
+  if ((la.group_rows == nullptr && la.G != 1) || static_cast<long long>(la.G) * la.N > 0x7fffffffll) return -12;
+  const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
+  if (gated && la.N % 256 != 0) return -13;
+  if (la.n_out != (la.mode != LIN_FORWARD ? la.K : gated ? la.N / 2 : la.N)) return -14;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // rows of tiles that share a stretch of the weights while it is in L2: about 48 MB of the row operand, at most 16 tiles
+  const long long tile_bytes = static_cast<long long>(la.pair ? 2 * LBM : LBM) * (la.mode == LIN_DX ? la.N : la.K) * 2;
+  const long long gm = (48ll << 20) / tile_bytes;
+  la.group_m = static_cast<int>(gm < 1 ? 1 : gm > 16 ? 16 : gm);
+  switch (la.mode) {
+    case LIN_FORWARD:
+      if (gated) return la.pair ? linear_launch<LIN_FORWARD, 2, true>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, true>(la, ctas, st);
+      return la.pair ? linear_launch<LIN_FORWARD, 2, false>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, false>(la, ctas, st);
+    case LIN_DX: return la.pair ? linear_launch<LIN_DX, 2, false>(la, ctas, st) : linear_launch<LIN_DX, 1, false>(la, ctas, st);
+    case LIN_DW: return la.pair ? linear_launch<LIN_DW, 2, false>(la, ctas, st) : linear_launch<LIN_DW, 1, false>(la, ctas, st);
+  }
+  return -15;
+}
+
+int b200_act_grad(const b200_act_grad_args* args, void* stream) {
+  using namespace b200;
+  if (args == nullptr || args->G < 1 || args->M < 1 || args->N < 8 || args->N % 8 != 0 || args->chunk_rows < 1 ||
+      static_cast<long long>(args->chunks) * args->chunk_rows < args->M || (args->group_rows == nullptr && args->G != 1))
+    return -10;
+  if (args->dbias != nullptr && args->record == nullptr) return -11;
+  if ((args->act != ACT_NONE) != (args->z != nullptr) || (args->z != nullptr) != (args->dz != nullptr)) return -12;
+  if (args->elem != ELEM_BF16 && args->elem != ELEM_F16) return -13;
+  const b200_act_grad_args& a = *args;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
+  b200_count_launches(1);
+  if (a.elem == ELEM_BF16) act_grad_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
+  else act_grad_kernel<__half><<<grid, 128, 0, st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.dbias == nullptr) return static_cast<int>(e);
+  b200_count_launches(1);
+  const dim3 fin((a.N + 255) / 256, a.G);
+  if (a.elem == ELEM_BF16) e = launch_chained(bias_grad_kernel<__nv_bfloat16>, fin, dim3(256), 0, st, a);
+  else e = launch_chained(bias_grad_kernel<__half>, fin, dim3(256), 0, st, a);
+  return static_cast<int>(e);
+}
+
+void b200_abi_sizes_linear(int* out) {
+  out[0] = static_cast<int>(sizeof(b200_linear_args));
+  out[1] = static_cast<int>(sizeof(b200_act_grad_args));
+}
+
+}  // extern "C"

@@ -222,6 +222,25 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, WaitCt
   return true;
 }
 
+// The same for a barrier on which other CTAs of the cluster arrive after writing data that the waiter goes on to use.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, WaitCtx& w, int code) {
+  if (!mbar_wait(bar, parity, w, code)) return false;
+  return mbar_try_wait_cluster(bar, parity);      // completed: acquires at cluster scope
+}
+
 // ----------------------------------------------------------------------------
 // Programmatic dependent launch.  A kernel launched with launch_chained (launch.h) may start while its
 // predecessor in the stream still runs: before chain_wait() it touches nothing that an earlier kernel
@@ -254,6 +273,14 @@ __device__ __forceinline__ void tma_load_2d_hint(void* smem_dst, const void* tma
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
       " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(smem_dst)),
       "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
+      : "memory");
+}
+// The same of a 3-D map (x innermost).
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 // L2 eviction priorities for streamed / reused operands.
@@ -431,6 +458,14 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const void* tma
       "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int x,
+                                                 int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_2d_pair_hint(void* smem_dst, const void* tmap,
                                                       uint32_t bar_cluster_addr, int x, int y,
                                                       uint64_t policy) {
@@ -488,6 +523,19 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for an MN-major tile: boxes of 64 elements along M or N by BK steps along K, one behind the other.  A row of
+// a box (128 bytes, swizzled as above) is one step of K; eight steps form an atom (SBO: the next eight steps) and
+// LBO is the distance of two boxes.  16 steps of K are 2048 bytes.
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_addr, uint32_t box_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(box_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
 // Instruction descriptor for kind::f16, bf16 x bf16 -> fp32, both operands
 // K-major, dense, no negation.
 __host__ __device__ constexpr uint32_t make_idesc_bf16_f32(int M, int N) {
@@ -496,6 +544,12 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16_f32(int M, int N) {
          | (1u << 10)                                // B format: BF16
          | (static_cast<uint32_t>(N >> 3) << 17)     // N / 8
          | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
+}
+
+// kind::f16 with both operands bf16 or both fp16; a set `mn` bit: that operand is MN-major (transposed).
+__host__ __device__ constexpr uint32_t make_idesc_16bit(int M, int N, bool bf16, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
+         ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {

@@ -7,6 +7,7 @@ from .balance import balance_loss
 from .combine import padded_return, weighted_gather
 from .dispatch import AllToAllOp, custom_a2a, zero_padding
 from .expert import Expert, expert, grouped_gemm, to_kmajor
+from .linear import linear
 from .norm import post_norm, pre_norm
 from .plan import Plan, make_plan, pack_rows
 from .router import router_topk

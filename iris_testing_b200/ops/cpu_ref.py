@@ -282,3 +282,30 @@ def balance_loss_ref(logits: torch.Tensor, topk_idx: torch.Tensor, balance_coef:
     terms = E * (counts.to(lg.dtype) * prob).sum(1) / (k * some * some)
     z = torch.logsumexp(lg, 1).pow(2).sum() / max(t.numel(), 1)
     return balance_coef * terms.sum() / max(int((n_s > 0).sum()), 1) + z_coef * z, counts.to(torch.int32)
+
+
+def linear_ref(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+               activation: Optional[str], group_rows: Optional[torch.Tensor]) -> torch.Tensor:
+    """act(x @ w.T + bias) + residual per group of packed rows, unrounded; rows behind the last group are zero."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    rows = [x.shape[0]] if group_rows is None else group_rows.clamp(min=0).tolist()
+    w = w if w.dim() == 3 else w.unsqueeze(0)
+    parts, start = [], 0
+    for g, n in enumerate(rows):
+        z = x[start:start + n].to(wide) @ w[g].to(wide).t()
+        if bias is not None:
+            z = z + bias.reshape(w.shape[0], -1)[g].to(wide)
+        if activation == "relu":
+            z = F.relu(z)
+        elif activation == "silu":
+            z = F.silu(z)
+        elif activation == "gelu":
+            z = F.gelu(z, approximate="tanh")
+        elif activation == "silu_gate":
+            v = z.unflatten(1, (-1, 2, 128))
+            z = (F.silu(v[:, :, 0]) * v[:, :, 1]).flatten(1)
+        if residual is not None:
+            z = z + residual[start:start + n].to(wide)
+        parts.append(z)
+        start += n
+    return torch.cat(parts + [parts[0].new_zeros(x.shape[0] - start, parts[0].shape[1])])

@@ -1,0 +1,180 @@
+"""Matrix product with bias, activation and residual in its epilogue, dense (a shared expert, a projection) or with one
+weight per expert over packed ragged rows, with its gradients.
+
+``grouped_gemm`` is the plain product of the expert path, forward only; the reference's expert is forward only too
+(layers/expert.py:6-65).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from .. import _native as nv
+from . import cpu_ref
+from ._common import ELEM, declare, launch_status, on_device, require, require_device, require_elem, stream_ptr, use_native
+from .expert import pairs_pay, sm_count
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
+_FORWARD, _DX, _DW = 0, 1, 2
+_BIAS_CHUNK = 64          # rows whose sum is one record of the bias gradient
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("a", "b", "out", "z", "bias", "res", "group_rows", "status")] \
+        + [("wait_budget_ns", C.c_ulonglong)] \
+        + [(n, C.c_int) for n in ("mode", "G", "M", "N", "K", "n_out", "elem", "act", "pair", "group_m")]
+
+
+class ActGradArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "dz", "dres", "dbias", "record", "group_rows")] \
+        + [(n, C.c_int) for n in ("G", "M", "N", "n_out", "elem", "act", "chunks", "chunk_rows")]
+
+
+def _plain(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and starting on 16 bytes, by a copy where it is not."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _pairs(mode: int, M: int, N: int, K: int, G: int) -> bool:
+    """Whether a tile is shared by two CTAs."""
+    if mode == _DW:
+        return G * -(-N // 256) * -(-K // 256) >= 74
+    return pairs_pay(M / G)
+
+
+def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, res=None):
+    la = LinearArgs()
+    la.a, la.b, la.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
+    la.z = None if z is None else z.data_ptr()
+    la.bias = None if bias is None else bias.data_ptr()
+    la.res = None if res is None else res.data_ptr()
+    la.group_rows = None if group_rows is None else group_rows.data_ptr()
+    la.status = launch_status(a.device).data_ptr()
+    la.wait_budget_ns = 2_000_000_000
+    la.mode, la.G, la.M, la.N, la.K, la.n_out = mode, G, M, N, K, out.shape[-1]
+    la.elem, la.act, la.pair = ELEM[a.dtype], act, int(_pairs(mode, M, N, K, G))
+    fn = declare("b200_linear", [C.POINTER(LinearArgs), C.c_int, C.c_void_p])
+    nv.check(fn(C.byref(la), sm_count(a.device), stream_ptr(a)), "linear launch")
+
+
+def _forward(x, w, bias, residual, group_rows, act, save):
+    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain."""
+    M, K = x.shape
+    G, N = (1, w.shape[0]) if w.dim() == 2 else w.shape[:2]
+    n_out = N // 2 if act == 4 else N
+    y = torch.empty((M, n_out), dtype=x.dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save and act else None
+    if M > 0:
+        with on_device(x):
+            _product(_FORWARD, x, w, y, M, N, K, G, group_rows, act, z, bias, residual)
+    return y, z
+
+
+def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
+    M, K = x.shape
+    G, N = (1, w.shape[0]) if w.dim() == 2 else w.shape[:2]
+    dev, dt = x.device, x.dtype
+    dx = torch.empty_like(x) if need[0] else None
+    dw = torch.empty_like(w) if need[1] else None
+    db = torch.empty((G, N) if w.dim() == 3 else (N,), dtype=dt, device=dev) if has_bias and need[2] else None
+    dres = None
+    if has_res and need[3]:                  # without groups every row of dy is the residual's gradient as it is
+        dres = dy if group_rows is None else torch.empty_like(dy)
+    if M == 0:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), dres
+    own_dres = dres is not None and dres is not dy
+    with on_device(x):
+        dz = dy
+        if db is not None or own_dres or (act and (need[0] or need[1])):
+            a = ActGradArgs()
+            if act:
+                dz = torch.empty((M, N), dtype=dt, device=dev)
+                a.z, a.dz = z.data_ptr(), dz.data_ptr()
+            a.dy = dy.data_ptr()
+            a.dres = dres.data_ptr() if own_dres else None
+            a.G, a.M, a.N, a.n_out, a.elem, a.act = G, M, N, dy.shape[1], ELEM[dt], act
+            a.group_rows = None if group_rows is None else group_rows.data_ptr()
+            a.chunk_rows, a.chunks = _BIAS_CHUNK, -(-M // _BIAS_CHUNK)
+            if db is not None:
+                record = torch.empty((a.chunks + G, N), dtype=torch.float32, device=dev)
+                a.dbias, a.record = db.data_ptr(), record.data_ptr()
+            fn = declare("b200_act_grad", [C.POINTER(ActGradArgs), C.c_void_p])
+            nv.check(fn(C.byref(a), stream_ptr(x)), "activation gradient launch")
+        if dx is not None:
+            _product(_DX, dz, w, dx, M, N, K, G, group_rows)
+        if dw is not None:
+            _product(_DW, dz, x, dw, M, N, K, G, group_rows)
+    return dx, dw, db, dres
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, group_rows, act):
+        y, z = _forward(x, w, bias, residual, group_rows, act, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, w, z, group_rows)
+        ctx.how = (bias is not None, residual is not None, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, z, group_rows = ctx.saved_tensors
+        has_bias, has_res, act = ctx.how
+        return (*_backward(x, w, z, has_bias, has_res, group_rows, act, ctx.needs_input_grad[:4], _plain(dy)), None, None)
+
+
+def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           residual: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
+           group_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ w.T + bias) + residual`` in x's dtype; differentiable by x, w, bias and residual.
+
+    x           [..., K] bfloat16 or float16 (with ``group_rows``: [M, K], the groups' rows packed one after another)
+    w_kmajor    [N, K], or with ``group_rows`` [G, N, K] (:func:`to_kmajor`), G <= 128
+    bias        [N] or [G, N];  residual [..., n_out]: what is added after the activation
+    activation  None, "relu", "silu", "gelu" (tanh form), or "silu_gate": every 256 rows of w hold 128 gate rows and
+                then 128 up rows, the result is silu(gate) * up and n_out = N / 2
+    group_rows  int32 [G] on x's device: rows of each group, none allowed.  Rows of x behind the last group are not read;
+                the result and the gradients of x and residual are zero there.
+
+    All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; a backward pass keeps the
+    pre-activation and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
+    timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.  CPU tensors take
+    plain PyTorch."""
+    require(activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)} (got {activation!r})")
+    grouped = group_rows is not None
+    require(w_kmajor.dim() == (3 if grouped else 2), "w_kmajor must be [N, K], or [G, N, K] with group_rows")
+    N, K = w_kmajor.shape[-2:]
+    require(x.dim() >= 1 and x.shape[-1] == K and (x.dim() == 2 or not grouped),
+            "x must be [..., K], or [M, K] with group_rows")
+    require(N >= 1 and K >= 1, "w_kmajor must have rows and columns")
+    act = ACTIVATIONS[activation]
+    require(act != 4 or N % 256 == 0, "silu_gate needs N (= 2 * n_out) to be a multiple of 256")
+    n_out = N // 2 if act == 4 else N
+    G = w_kmajor.shape[0] if grouped else 1
+    require(bias is None or bias.shape == ((G, N) if grouped else (N,)), "bias must have one value per row of w_kmajor")
+    require(residual is None or residual.shape == x.shape[:-1] + (n_out,), "residual must have the result's shape")
+    require(not grouped or (group_rows.dtype == torch.int32 and group_rows.shape == (G,)),
+            "group_rows must be int32 with one entry per group")
+    require(not grouped or 1 <= G <= nv.MAX_GROUPS, f"at most {nv.MAX_GROUPS} groups")
+    shape = x.shape[:-1] + (n_out,)
+    if not use_native(x):
+        require(not grouped or int(group_rows.clamp(min=0).sum()) <= x.shape[0], "the groups hold more rows than x")
+        r = None if residual is None else residual.reshape(-1, n_out)
+        return cpu_ref.linear_ref(x.reshape(-1, K), w_kmajor, bias, r, activation, group_rows).to(x.dtype).view(shape)
+    require_elem(x, "x", (torch.bfloat16, torch.float16))
+    for name, t in (("w_kmajor", w_kmajor), ("bias", bias), ("residual", residual)):
+        require(t is None or t.dtype == x.dtype, f"{name} must have x's dtype")
+    require(K % 8 == 0 and N % 8 == 0, "K and N must be multiples of 8")
+    require(x.numel() // K < 2 ** 31 and G * N < 2 ** 31, "too many rows")
+    require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)
+    x2 = _plain(x.reshape(-1, K))
+    r2 = None if residual is None else _plain(residual.reshape(-1, n_out))
+    w, b = _plain(w_kmajor), _plain(bias)
+    rows = None if group_rows is None else group_rows.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_kmajor, bias, residual)):
+        return _Linear.apply(x2, w, b, r2, rows, act).view(shape)
+    return _forward(x2, w, b, r2, rows, act, False)[0].view(shape)
