@@ -10,8 +10,8 @@
 // not counted) behind the last sequence, where the mask is false, and where its logits have no usable maximum: a NaN,
 // +infinity, or none above the type's lowest value (every expert masked).
 //
-// A block takes a run of tokens and walks the sequences in it one after another; 2^x lanes share a token.  Column
-// sums stay in registers until the sequence or the run ends; then one record per (run, sequence) is written: sums of p,
+// A block takes a run of tokens and walks the sequences in it one after another; 2^x lanes share a token, each with whole
+// packs of 16 bytes of its logits, and hold the next token's while they work on one.  Column sums stay in registers until the sequence or the run ends; then one record per (run, sequence) is written: sums of p,
 // counts, tokens, sum of lse^2.  Runs and sequences only ever advance, so run + sequence numbers the records
 // without gaps.  A second kernel adds a sequence's records in their order.  No atomics on floating-point values: the same
 // inputs give the same bits.
@@ -33,7 +33,8 @@ typedef struct b200_balance_args {
   int* counts;               // [S, E]
   int* kept;                 // [S, E]: the same again, for the backward pass (the caller may change its own)
   float* record;             // [runs + S][2 E + 2]: sums of p, counts (int), tokens (int), sum of lse^2
-  float* seq_loss;           // [S][2]: a sequence's balance term, its sum of lse^2
+  float* seq_loss;           // [S][ceil(E / 32)]: 32 experts' part of a sequence's term
+  float* seq_z;              // [S]: its sum of lse^2
   int* seq_tokens;           // [S]
   float* total;              // [2]: 1 / S' (0 without a token), 1 / n
   int* ticket;               // [1]
@@ -94,48 +95,80 @@ __device__ __forceinline__ void find_sequence(const b200_balance_args& a, long l
   start = found_start;
 }
 
-// One token's softmax over the lanes that share it: p[i] for expert i * LPT + sub.  False: it takes no part.
-template <typename T, int LPT, int C>
-__device__ __forceinline__ bool token_softmax(const b200_balance_args& a, long long t, bool in, int sub, float (&p)[C], float& lse) {
-  if (in && a.mask != nullptr) in = a.mask[t] != 0;
-  const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-  float mx = -CUDART_INF_F;
-  bool ok = true;
+// How a token's experts lie on the LPT lanes that share it: P packs of V logits per lane; value i of a lane is expert
+// expert_of(i, sub).  V is 1 where rows do not start on 16 bytes.
+template <int LPT, int V>
+__device__ __forceinline__ int expert_of(int i, int sub) { return (i / V * LPT + sub) * V + i % V; }
+
+template <typename T, int V, int P>
+struct TokenRow {
+  Pack<T, V> k[P];
+};
+
+template <typename T> __device__ __forceinline__ T minus_infinity();
+template <> __device__ __forceinline__ float minus_infinity<float>() { return -CUDART_INF_F; }
+template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+template <> __device__ __forceinline__ __half minus_infinity<__half>() { return __ushort_as_half(0xfc00); }
+
+// Loads one token's logits; minus infinity behind the last expert, and everywhere where `in` is false.
+template <typename T, int LPT, int V, int P>
+__device__ __forceinline__ void load_token(const b200_balance_args& a, long long t, bool in, int sub, TokenRow<T, V, P>& row) {
+  const T* p = static_cast<const T*>(a.logits) + t * a.ld;
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    const int e = i * LPT + sub;
-    p[i] = in && e < a.E ? to_f32(row[e]) : -CUDART_INF_F;
-    ok = ok && !(p[i] != p[i]);
-    mx = fmaxf(mx, p[i]);
+  for (int i = 0; i < P; ++i) {
+    const int e = (i * LPT + sub) * V;
+    if (in && e < a.E) row.k[i] = *reinterpret_cast<const Pack<T, V>*>(p + e);
+    else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) row.k[i].v[j] = minus_infinity<T>();
+    }
+  }
+}
+
+// One token's exponentials over the lanes that share it and the inverse of their sum.  False: it takes no part.
+// exp(l - max) is 2^(l log2 e - m) with m = max log2 e rounded once per token: the shift is the same for every expert, so
+// its rounding has no part in p, and lse is m ln 2 + log(sum).
+template <typename T, int LPT, int V, int P>
+__device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, float (&p)[V * P], float& inv, float& lse) {
+  constexpr int C = V * P;
+  float mx = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    float x[V];
+    unpack<T, V>(row.k[i], x);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      p[i * V + j] = x[j];
+      mx = max_nan(mx, x[j]);
+    }
   }
 #pragma unroll
-  for (int o = LPT / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  ok = ok && mx > lowest<T>() && mx < CUDART_INF_F;
-  // every lane of the token has to have seen no NaN
-  const unsigned all = __ballot_sync(0xffffffffu, ok);
-  const unsigned mine = (LPT == 32 ? 0xffffffffu : ((1u << LPT) - 1u) << ((threadIdx.x & 31) / LPT * LPT));
-  ok = (all & mine) == mine;
+  for (int o = LPT / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const bool ok = mx > lowest<T>() && mx < CUDART_INF_F;      // no for a NaN
+  const float m = mx * LOG2_E;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    p[i] = ok ? expf(p[i] - mx) : 0.f;
+    p[i] = exp2_approx(fmaf(p[i], LOG2_E, -m));
     sum += p[i];
   }
 #pragma unroll
   for (int o = LPT / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = ok ? 1.f / sum : 0.f;
+  if (!ok) {
 #pragma unroll
-  for (int i = 0; i < C; ++i) p[i] *= inv;
-  lse = ok ? mx + logf(sum) : 0.f;
+    for (int i = 0; i < C; ++i) p[i] = 0.f;
+  }
+  inv = ok ? 1.f / sum : 0.f;
+  lse = ok ? fmaf(m, LN_2, __logf(sum)) : 0.f;
   return ok;
 }
 
-template <typename T, int LPT, int C>
+template <typename T, int LPT, int V, int P>
 __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200_balance_args a) {
   extern __shared__ float sm[];              // [warps][E] sums of p, then int [E] counts
   __shared__ float warp_z[BAL_THREADS / 32];
   __shared__ int warp_n[BAL_THREADS / 32];
-  constexpr int WARPS = BAL_THREADS / 32, TOK = 32 / LPT;
+  constexpr int WARPS = BAL_THREADS / 32, TOK = 32 / LPT, C = V * P;
   int* cnt = reinterpret_cast<int*>(sm + WARPS * a.E);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPT, slot = lane / LPT;
   const long long t0 = static_cast<long long>(blockIdx.x) * a.run_tokens;
@@ -156,25 +189,32 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200
     for (int i = 0; i < C; ++i) col[i] = 0.f;
     float zsum = 0.f;
     int tokens = 0;
-    for (long long t = pos + warp * TOK; t < end; t += WARPS * TOK) {
-      float p[C], lse;
-      const long long mine = t + slot;
-      const bool ok = token_softmax<T, LPT, C>(a, mine, mine < end, sub, p, lse);
-      if (!ok) continue;
+    long long t = pos + warp * TOK;
+    TokenRow<T, V, P> row, next;
+    auto takes = [&](long long at) { return at < end && (a.mask == nullptr || a.mask[at] != 0); };
+    load_token<T, LPT, V, P>(a, t + slot, takes(t + slot), sub, row);
+    for (; t < end; t += WARPS * TOK) {
+      const long long mine = t + slot, after = mine + WARPS * TOK;
+      load_token<T, LPT, V, P>(a, after, takes(after), sub, next);
+      float p[C], inv, lse;
+      const bool ok = token_softmax<T, LPT, V, P>(row, p, inv, lse);
 #pragma unroll
-      for (int i = 0; i < C; ++i) col[i] += p[i];
-      for (int j = sub; j < a.k; j += LPT) {
-        const int e = a.idx[mine * a.k + j];
-        if (e >= 0 && e < a.E) atomicAdd(cnt + e, 1);
+      for (int i = 0; i < C; ++i) col[i] = fmaf(p[i], inv, col[i]);
+      if (ok) {
+        for (int j = sub; j < a.k; j += LPT) {
+          const int e = a.idx[mine * a.k + j];
+          if (e >= 0 && e < a.E) atomicAdd(cnt + e, 1);
+        }
+        if (sub == 0) { zsum += lse * lse; ++tokens; }
       }
-      if (sub == 0) { zsum += lse * lse; ++tokens; }
+      row = next;
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < C; ++i) {
 #pragma unroll
       for (int o = LPT; o < 32; o <<= 1) col[i] += __shfl_xor_sync(0xffffffffu, col[i], o);
-      if (slot == 0 && i * LPT + sub < a.E) sm[warp * a.E + i * LPT + sub] = col[i];
+      if (slot == 0 && expert_of<LPT, V>(i, sub) < a.E) sm[warp * a.E + expert_of<LPT, V>(i, sub)] = col[i];
     }
     zsum = warp_sum(zsum);
     tokens = __reduce_add_sync(0xffffffffu, tokens);
@@ -200,64 +240,66 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200
   }
 }
 
-// One block per sequence: adds its records, writes its counts and its term; the last block adds the terms.
-__global__ void __launch_bounds__(BAL_THREADS) balance_finish_kernel(const b200_balance_args a) {
-  __shared__ float red[BAL_THREADS / 32];
-  __shared__ double dred[2][BAL_THREADS / 32];
-  __shared__ int nred[2][BAL_THREADS / 32];
-  __shared__ long long ired[BAL_THREADS / 32];
+// Block (s, c) adds the records of 32 experts of a sequence, each of 16 warps a share of the runs in their order, and
+// writes the counts and the experts' part of sum_e c_e P_e; the last block of all adds the parts.
+constexpr int FIN_WARPS = 16;
+__global__ void __launch_bounds__(FIN_WARPS * 32) balance_finish_kernel(const b200_balance_args a) {
+  __shared__ float sh_p[FIN_WARPS][33], sh_z[FIN_WARPS];
+  __shared__ int sh_c[FIN_WARPS][33], sh_n[FIN_WARPS];
+  __shared__ long long sh_start[FIN_WARPS];
+  __shared__ double sh_d[2][FIN_WARPS];
   __shared__ int last;
   chain_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int stride = 2 * a.E + 2;
-  for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
-    // tokens [start, start + len) lie in runs start / run_tokens ... ; record numbers are run + s
+  const int chunks = (a.E + 31) / 32, stride = 2 * a.E + 2;
+  for (int job = blockIdx.x; job < a.S * chunks; job += gridDim.x) {
+    const int s = job / chunks, e = (job - s * chunks) * 32 + lane;
     long long start = 0;
     if (a.seq_rows != nullptr) {
-      long long part = 0;
-      for (int q = tid; q < s; q += BAL_THREADS) part += max(0, a.seq_rows[q]);
+      for (int q = tid; q < s; q += FIN_WARPS * 32) start += max(0, a.seq_rows[q]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == 0) ired[warp] = part;
+      for (int o = 16; o > 0; o >>= 1) start += __shfl_xor_sync(0xffffffffu, start, o);
+      if (lane == 0) sh_start[warp] = start;
       __syncthreads();
-      for (int w = 0; w < BAL_THREADS / 32; ++w) start += ired[w];
-      __syncthreads();
+      start = 0;
+      for (int w = 0; w < FIN_WARPS; ++w) start += sh_start[w];
     }
+    // the runs that hold a token of s (none: nothing was recorded); record numbers are run + s
     const long long len = a.seq_rows != nullptr ? max(0, a.seq_rows[s]) : a.T;
     const long long end = min(static_cast<long long>(a.T), start + len);
-    // runs that hold a token of s; none: no record is read
     const int r0 = static_cast<int>(min(start, static_cast<long long>(a.T)) / a.run_tokens);
     const int r1 = end > start ? static_cast<int>((end - 1) / a.run_tokens) : r0 - 1;
-    int n = 0;
-    float z = 0.f;
-    for (int r = r0; r <= r1; ++r) {
+    float p = 0.f, z = 0.f;
+    int c = 0, n = 0;
+#pragma unroll 4
+    for (int r = r0 + warp; r <= r1; r += FIN_WARPS) {
       const float* rec = a.record + (static_cast<size_t>(r) + s) * stride;
-      n += reinterpret_cast<const int*>(rec)[2 * a.E];
-      z += rec[2 * a.E + 1];
-    }
-    float dot = 0.f;
-    for (int e = tid; e < a.E; e += BAL_THREADS) {
-      float p = 0.f;
-      int c = 0;
-      for (int r = r0; r <= r1; ++r) {
-        const float* rec = a.record + (static_cast<size_t>(r) + s) * stride;
+      if (e < a.E) {
         p += rec[e];
         c += reinterpret_cast<const int*>(rec)[a.E + e];
       }
-      a.counts[static_cast<size_t>(s) * a.E + e] = c;
-      a.kept[static_cast<size_t>(s) * a.E + e] = c;
-      dot += p * static_cast<float>(c);
+      n += reinterpret_cast<const int*>(rec)[2 * a.E];
+      z += rec[2 * a.E + 1];
     }
-    dot = warp_sum(dot);
-    if (lane == 0) red[warp] = dot;
+    sh_p[warp][lane] = p;
+    sh_c[warp][lane] = c;
+    if (lane == 0) { sh_z[warp] = z; sh_n[warp] = n; }
     __syncthreads();
-    if (tid == 0) {
-      float v = 0.f;
-      for (int w = 0; w < BAL_THREADS / 32; ++w) v += red[w];
-      const float nn = static_cast<float>(n);
-      a.seq_loss[2 * s] = n > 0 ? static_cast<float>(a.E) * (v / nn) / (static_cast<float>(a.k) * nn) : 0.f;
-      a.seq_loss[2 * s + 1] = z;
-      a.seq_tokens[s] = n;
+    if (warp == 0) {
+      for (int w = 1; w < FIN_WARPS; ++w) { p += sh_p[w][lane]; c += sh_c[w][lane]; z += sh_z[w]; n += sh_n[w]; }
+      if (e < a.E) {
+        a.counts[static_cast<size_t>(s) * a.E + e] = c;
+        a.kept[static_cast<size_t>(s) * a.E + e] = c;
+      }
+      const float dot = warp_sum(p * static_cast<float>(c));
+      if (lane == 0) {
+        const float nn = static_cast<float>(n);
+        a.seq_loss[job] = n > 0 ? static_cast<float>(a.E) * (dot / nn) / (static_cast<float>(a.k) * nn) : 0.f;
+        if (job == s * chunks) {
+          a.seq_z[s] = z;
+          a.seq_tokens[s] = n;
+        }
+      }
     }
     __syncthreads();
   }
@@ -268,11 +310,10 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_finish_kernel(const b200_
   if (!last) return;
   __threadfence();
   double sum = 0.0, zs = 0.0;
-  int full = 0;
-  long long tokens = 0;
-  for (int s = tid; s < a.S; s += BAL_THREADS) {
-    sum += __ldcg(a.seq_loss + 2 * s);
-    zs += __ldcg(a.seq_loss + 2 * s + 1);
+  int full = 0, tokens = 0;
+  for (int j = tid; j < a.S * chunks; j += FIN_WARPS * 32) sum += __ldcg(a.seq_loss + j);
+  for (int s = tid; s < a.S; s += FIN_WARPS * 32) {
+    zs += __ldcg(a.seq_z + s);
     const int n = __ldcg(a.seq_tokens + s);
     full += n > 0;
     tokens += n;
@@ -281,26 +322,22 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_finish_kernel(const b200_
   for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
     zs += __shfl_xor_sync(0xffffffffu, zs, o);
-    full += __shfl_xor_sync(0xffffffffu, full, o);
-    tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
   }
-  if (lane == 0) { dred[0][warp] = sum; dred[1][warp] = zs; nred[0][warp] = full; nred[1][warp] = static_cast<int>(tokens); }
+  full = __reduce_add_sync(0xffffffffu, full);
+  tokens = __reduce_add_sync(0xffffffffu, tokens);
+  if (lane == 0) { sh_d[0][warp] = sum; sh_d[1][warp] = zs; sh_c[warp][0] = full; sh_n[warp] = tokens; }
   __syncthreads();
   if (tid == 0) {
-    sum = zs = 0.0;
-    full = 0;
-    int n = 0;
-    for (int w = 0; w < BAL_THREADS / 32; ++w) { sum += dred[0][w]; zs += dred[1][w]; full += nred[0][w]; n += nred[1][w]; }
-    const float inv_s = full > 0 ? 1.f / static_cast<float>(full) : 0.f, inv_n = n > 0 ? 1.f / static_cast<float>(n) : 0.f;
-    *a.loss = full > 0 ? static_cast<float>(a.coef * sum / full + a.z * zs / n) : 0.f;
-    a.total[0] = inv_s;
-    a.total[1] = inv_n;
+    for (int w = 1; w < FIN_WARPS; ++w) { sum += sh_d[0][w]; zs += sh_d[1][w]; full += sh_c[w][0]; tokens += sh_n[w]; }
+    *a.loss = full > 0 ? static_cast<float>(a.coef * sum / full + a.z * zs / tokens) : 0.f;
+    a.total[0] = full > 0 ? 1.f / static_cast<float>(full) : 0.f;
+    a.total[1] = tokens > 0 ? 1.f / static_cast<float>(tokens) : 0.f;
   }
 }
 
-template <typename T, int LPT, int C>
+template <typename T, int LPT, int V, int P>
 __global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b200_balance_args a) {
-  constexpr int WARPS = BAL_THREADS / 32, TOK = 32 / LPT;
+  constexpr int WARPS = BAL_THREADS / 32, TOK = 32 / LPT, C = V * P;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPT, slot = lane / LPT;
   const long long t0 = static_cast<long long>(blockIdx.x) * a.run_tokens;
   const long long t1 = min(static_cast<long long>(a.T), t0 + a.run_tokens);
@@ -319,26 +356,36 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b20
     float coef[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int e = i * LPT + sub;
+      const int e = expert_of<LPT, V>(i, sub);
       coef[i] = n > 0 && e < a.E ? scale * static_cast<float>(a.kept[static_cast<size_t>(seq) * a.E + e]) : 0.f;
     }
-    for (long long t = pos + warp * TOK; t < end; t += WARPS * TOK) {
-      float p[C], lse;
-      const long long mine = t + slot;
-      const bool in = mine < end;
-      const bool ok = token_softmax<T, LPT, C>(a, mine, in && n > 0, sub, p, lse);
+    long long t = pos + warp * TOK;
+    TokenRow<T, V, P> row, next;
+    auto takes = [&](long long at) { return n > 0 && at < end && (a.mask == nullptr || a.mask[at] != 0); };
+    load_token<T, LPT, V, P>(a, t + slot, takes(t + slot), sub, row);
+    for (; t < end; t += WARPS * TOK) {
+      const long long mine = t + slot, after = mine + WARPS * TOK;
+      load_token<T, LPT, V, P>(a, after, takes(after), sub, next);
+      float p[C], inv, lse;
+      const bool ok = token_softmax<T, LPT, V, P>(row, p, inv, lse);
       float dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < C; ++i) dot += p[i] * coef[i];
+      for (int i = 0; i < C; ++i) dot = fmaf(p[i], coef[i], dot);
 #pragma unroll
       for (int o = LPT / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if (!in) continue;
-      T* out = static_cast<T*>(a.grad) + mine * a.E;
+      if (mine < end) {
+        T* out = static_cast<T*>(a.grad) + mine * a.E;
+        const float shift = zc * lse - dot * inv, scaled = ok ? g * inv : 0.f;      // an infinite g leaves other tokens at 0
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int e = i * LPT + sub;
-        if (e < a.E) out[e] = from_f32<T>(ok ? g * (p[i] * (coef[i] - dot) + zc * lse * p[i]) : 0.f);
+        for (int q = 0; q < P; ++q) {
+          const int e = (q * LPT + sub) * V;
+          float d[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] = scaled * p[q * V + j] * (coef[q * V + j] + shift);
+          if (e < a.E) store_pack<T, V>(out + e, d);
+        }
       }
+      row = next;
     }
     __syncwarp();
     pos = end;
@@ -347,32 +394,43 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b20
   }
 }
 
-template <bool BACK, typename T, int LPT, int C>
+template <bool BACK, typename T, int LPT, int V, int P>
 static cudaError_t balance_launch(const b200_balance_args& a, cudaStream_t st) {
   b200_count_launches(1);
   if constexpr (BACK) {
-    balance_backward_kernel<T, LPT, C><<<a.runs, BAL_THREADS, 0, st>>>(a);
+    balance_backward_kernel<T, LPT, V, P><<<a.runs, BAL_THREADS, 0, st>>>(a);
     return cudaGetLastError();
   } else {
     const size_t smem = (BAL_THREADS / 32 + 1) * static_cast<size_t>(a.E) * 4;      // 36 KB at 1024 experts
-    balance_forward_kernel<T, LPT, C><<<a.runs, BAL_THREADS, smem, st>>>(a);
+    balance_forward_kernel<T, LPT, V, P><<<a.runs, BAL_THREADS, smem, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     b200_count_launches(1);
-    return launch_chained(balance_finish_kernel, dim3(a.S < 592 ? a.S : 592), dim3(BAL_THREADS), 0, st, a);
+    const long long jobs = static_cast<long long>(a.S) * ((a.E + 31) / 32);
+    return launch_chained(balance_finish_kernel, dim3(static_cast<unsigned>(jobs < 592 ? jobs : 592)), dim3(FIN_WARPS * 32), 0, st, a);
   }
+}
+
+// Lanes per token: 16 experts a lane, so that a warp has several tokens in work and what is done once per token (shuffles,
+// addresses, counts) is shared; with 8 a lane the kernels took half as many instructions again.
+template <bool BACK, typename T, int V>
+static cudaError_t balance_lanes(const b200_balance_args& a, cudaStream_t st) {
+  constexpr int P = 16 / V;
+  if (a.E <= 8 && V > 1) return balance_launch<BACK, T, 1, V, 8 / V>(a, st);
+  if (a.E <= 16) return balance_launch<BACK, T, 1, V, P>(a, st);
+  if (a.E <= 32) return balance_launch<BACK, T, 2, V, P>(a, st);
+  if (a.E <= 64) return balance_launch<BACK, T, 4, V, P>(a, st);
+  if (a.E <= 128) return balance_launch<BACK, T, 8, V, P>(a, st);
+  if (a.E <= 256) return balance_launch<BACK, T, 16, V, P>(a, st);
+  if (a.E <= 512) return balance_launch<BACK, T, 32, V, P>(a, st);
+  return balance_launch<BACK, T, 32, V, 2 * P>(a, st);
 }
 
 template <bool BACK, typename T>
 static cudaError_t balance_dispatch(const b200_balance_args& a, cudaStream_t st) {
-  if (a.E <= 4) return balance_launch<BACK, T, 1, 4>(a, st);
-  if (a.E <= 8) return balance_launch<BACK, T, 2, 4>(a, st);
-  if (a.E <= 16) return balance_launch<BACK, T, 4, 4>(a, st);
-  if (a.E <= 32) return balance_launch<BACK, T, 8, 4>(a, st);
-  if (a.E <= 64) return balance_launch<BACK, T, 16, 4>(a, st);
-  if (a.E <= 128) return balance_launch<BACK, T, 32, 4>(a, st);
-  if (a.E <= 256) return balance_launch<BACK, T, 32, 8>(a, st);
-  return balance_launch<BACK, T, 32, 32>(a, st);
+  constexpr int V = 16 / sizeof(T);
+  const bool aligned = a.E % V == 0 && a.ld % V == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  return aligned ? balance_lanes<BACK, T, V>(a, st) : balance_lanes<BACK, T, 1>(a, st);
 }
 
 template <bool BACK>
@@ -396,14 +454,13 @@ extern "C" {
 int b200_balance_forward(const b200_balance_args* a, void* stream) { return b200::balance_run<false>(a, stream); }
 int b200_balance_backward(const b200_balance_args* a, void* stream) { return b200::balance_run<true>(a, stream); }
 
-// Blocks (runs of tokens) of a call: as many as fill the GPU four times over, but no fewer tokens each than the
-// warps of a block take in one turn.
-int b200_balance_runs(int T, int E, int sms) {
-  int lanes = 1;
-  while (lanes < 32 && lanes * 4 < E) lanes *= 2;
-  const int turn = b200::BAL_THREADS / lanes;
-  const int want = (T + turn - 1) / turn, most = 4 * sms;
-  return want < most ? want : most;
+// Blocks (runs of tokens) of a call: as many as fill the GPU four times over, but no shorter than 32 KB of logits (a
+// record is written and read per run).
+int b200_balance_runs(int T, int E, int elem, int sms) {
+  const long long bytes = static_cast<long long>(T) * E * (elem == b200::ELEM_F32 ? 4 : 2);
+  const long long want = (bytes + 32767) / 32768, most = 4ll * sms;
+  const long long runs = want < most ? want : most;
+  return static_cast<int>(runs < T ? runs : T);
 }
 
 int b200_abi_size_balance_args() { return static_cast<int>(sizeof(b200_balance_args)); }

@@ -109,26 +109,31 @@ constexpr int lin_smem() {
 static_assert(lin_smem<LIN_FORWARD, 1>() <= 232448 && lin_smem<LIN_FORWARD, 2>() <= 232448 && lin_smem<LIN_DW, 1>() <= 232448 &&
                   lin_smem<LIN_DW, 2>() <= 232448, "exceeds 227 KiB of shared memory per CTA");
 
-// 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-constexpr float GELU_A = 0.7978845608028654f, GELU_B = 0.044715f;    // tanh form: v * sigmoid(2 A (v + B v^3))
+// q = 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.f + exp2_approx(-LOG2_E * v)); }
+// The same with exp(-v) q = 1 - q beside it; the exponent is held where the exponential is finite.
+__device__ __forceinline__ void sigmoid_both(float minus_v_log2e, float& q, float& rest) {
+  const float e = exp2_approx(fminf(minus_v_log2e, 100.f));
+  q = rcp_approx(1.f + e);
+  rest = e * q;
+}
+constexpr float GELU_A = 2.f * 0.7978845608028654f, GELU_B = GELU_A * 0.044715f;    // tanh form: v * sigmoid(A v + B v^3)
 __device__ __forceinline__ float act_value(float v, int act) {
   if (act == ACT_RELU) return v < 0.f ? 0.f : v;
   if (act == ACT_SILU) return v * sigmoid_f(v);
-  if (act == ACT_GELU) return v * sigmoid_f(2.f * GELU_A * (v + GELU_B * v * v * v));
+  if (act == ACT_GELU) return v * sigmoid_f(v * fmaf(GELU_B, v * v, GELU_A));
   return v;
 }
 __device__ __forceinline__ float act_slope(float v, int act) {
   if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
+  float q, rest;
   if (act == ACT_SILU) {
-    const float q = sigmoid_f(v);
-    return q * (1.f + v * (1.f - q));
+    sigmoid_both(-LOG2_E * v, q, rest);
+    return q * fmaf(v, rest, 1.f);
   }
-  if (act == ACT_GELU) {
-    const float q = sigmoid_f(2.f * GELU_A * (v + GELU_B * v * v * v));
-    return q + v * q * (1.f - q) * 2.f * GELU_A * (1.f + 3.f * GELU_B * v * v);
-  }
-  return 1.f;
+  const float vv = v * v;
+  sigmoid_both(v * fmaf(-LOG2_E * GELU_B, vv, -LOG2_E * GELU_A), q, rest);
+  return q * fmaf(v * fmaf(3.f * GELU_B, vv, GELU_A), rest, 1.f);
 }
 
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
@@ -583,67 +588,86 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   }
 }
 
-// dz = act'(z) dy and the column sums of dz over each group.  A block takes eight columns per thread of a run of rows;
-// the sums of a (run, group) go to record run + group (both only ever advance), added up in order by the next kernel.
-template <typename T>
-__global__ void __launch_bounds__(128) act_grad_kernel(const b200_act_grad_args a) {
-  const bool gated = a.act == ACT_SILU_GATE;
-  // a thread's eight columns of the output; of the gated form they belong to eight columns of the gate and of the up half
+// dz = act'(z) dy and the column sums of dz over each group.  A thread takes eight columns of the output down a run of
+// rows, the next row under way while it works on one; the sums of a (run, group) go to record run + group (both only ever
+// advance), added up in order by the next kernel.  Bound by memory traffic with SUMS off; 64 registers, so that an SM holds
+// 1024 threads.
+template <typename T, bool GATED, bool SUMS>
+__global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_args a) {
+  using P = Pack<T, 8>;
+  // of the gated form, a thread's columns belong to eight columns of the gate and of the up half
   const int oc = (blockIdx.y * 128 + threadIdx.x) * 8;
-  const bool in = oc < a.n_out;
-  const int zc = gated ? (oc / 128) * 256 + oc % 128 : oc;
+  if (oc >= a.n_out) return;
+  const int zc = GATED ? (oc / 128) * 256 + oc % 128 : oc;
   long long start = 0;
   int g = 0;
-  const long long r0 = static_cast<long long>(blockIdx.x) * a.chunk_rows, r1 = min(static_cast<long long>(a.M), r0 + a.chunk_rows);
+  const long long first = static_cast<long long>(blockIdx.x) * a.chunk_rows, r1 = min(static_cast<long long>(a.M), first + a.chunk_rows);
   auto rows_of = [&](int i) { return a.group_rows != nullptr ? max(0, a.group_rows[i]) : a.M; };
-  while (g < a.G && start + rows_of(g) <= r0) start += rows_of(g++);
-  long long pos = r0;
+  while (g < a.G && start + rows_of(g) <= first) start += rows_of(g++);
+  const T* dy = static_cast<const T*>(a.dy) + oc;
+  const T* z = static_cast<const T*>(a.z) + zc;
+  const bool active = a.z != nullptr;
+  long long pos = first;
   for (; g < a.G && pos < r1; ++g) {
     const long long end = min(r1, start + rows_of(g));
     start += rows_of(g);
     if (end <= pos) continue;
     float sum[8], sum2[8];
+    if constexpr (SUMS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum[j] = sum2[j] = 0.f;
-    if (in) {
-      for (long long r = pos; r < end; ++r) {
-        float d[8], z[8], u[8];
-        load_pack<T, 8>(static_cast<const T*>(a.dy) + r * a.n_out + oc, d);
-        if (a.dres != nullptr) store_pack<T, 8>(static_cast<T*>(a.dres) + r * a.n_out + oc, d);
-        if (a.z != nullptr) {
-          load_pack<T, 8>(static_cast<const T*>(a.z) + r * a.N + zc, z);
-          if (gated) {
-            load_pack<T, 8>(static_cast<const T*>(a.z) + r * a.N + zc + 128, u);
+      for (int j = 0; j < 8; ++j) sum[j] = sum2[j] = 0.f;
+    }
+    P kd, kz, ku;
+    auto load = [&](long long r) {
+      kd = *reinterpret_cast<const P*>(dy + r * a.n_out);
+      if (active) kz = *reinterpret_cast<const P*>(z + r * a.N);
+      if (GATED) ku = *reinterpret_cast<const P*>(z + r * a.N + 128);
+    };
+    load(pos);
+    for (long long r = pos; r < end; ++r) {
+      const P cd = kd, cz = kz, cu = ku;
+      if (r + 1 < end) load(r + 1);
+      if (a.dres != nullptr) *reinterpret_cast<P*>(static_cast<T*>(a.dres) + r * a.n_out + oc) = cd;
+      float d[8], v[8];
+      unpack<T, 8>(cd, d);
+      if (active) {
+        T* dz = static_cast<T*>(a.dz) + r * a.N + zc;
+        unpack<T, 8>(cz, v);
+        if constexpr (GATED) {
+          float u[8], du[8];
+          unpack<T, 8>(cu, u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float q = sigmoid_f(z[j]);
-              const float du = d[j] * z[j] * q;
-              d[j] *= u[j] * q * (1.f + z[j] * (1.f - q));
-              u[j] = du;
-              sum2[j] += du;
-            }
-            store_pack<T, 8>(static_cast<T*>(a.dz) + r * a.N + zc + 128, u);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] *= act_slope(z[j], a.act);
+          for (int j = 0; j < 8; ++j) {
+            float q, rest;
+            sigmoid_both(-LOG2_E * v[j], q, rest);
+            const float dq = d[j] * q;
+            du[j] = dq * v[j];
+            d[j] = dq * u[j] * fmaf(v[j], rest, 1.f);
+            if constexpr (SUMS) sum2[j] += du[j];
           }
-          store_pack<T, 8>(static_cast<T*>(a.dz) + r * a.N + zc, d);
+          store_pack<T, 8>(dz + 128, du);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] *= act_slope(v[j], a.act);
         }
+        store_pack<T, 8>(dz, d);
+      }
+      if constexpr (SUMS) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += d[j];
       }
-      if (a.dbias != nullptr) {
-        float* rec = a.record + (static_cast<size_t>(blockIdx.x) + g) * a.N;
+    }
+    if constexpr (SUMS) {
+      float* rec = a.record + (static_cast<size_t>(blockIdx.x) + g) * a.N + zc;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          rec[zc + j] = sum[j];
-          if (gated) rec[zc + 128 + j] = sum2[j];
-        }
+      for (int j = 0; j < 8; ++j) {
+        rec[j] = sum[j];
+        if (GATED) rec[128 + j] = sum2[j];
       }
     }
     pos = end;
   }
-  if (a.dres != nullptr && in) {
+  if (a.dres != nullptr) {
     const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (long long r = pos; r < r1; ++r) store_pack<T, 8>(static_cast<T*>(a.dres) + r * a.n_out + oc, none);
   }
@@ -747,6 +771,17 @@ static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) 
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tz, la));
 }
 
+template <typename T>
+static cudaError_t act_grad_launch(const b200_act_grad_args& a, cudaStream_t st) {
+  const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
+  const bool gated = a.act == ACT_SILU_GATE, sums = a.dbias != nullptr;
+  auto kern = gated ? (sums ? act_grad_kernel<T, true, true> : act_grad_kernel<T, true, false>)
+                    : (sums ? act_grad_kernel<T, false, true> : act_grad_kernel<T, false, false>);
+  b200_count_launches(1);
+  kern<<<grid, 128, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
 }  // namespace b200
 
 extern "C" {
@@ -785,14 +820,11 @@ int b200_act_grad(const b200_act_grad_args* args, void* stream) {
   if (args->elem != ELEM_BF16 && args->elem != ELEM_F16) return -13;
   const b200_act_grad_args& a = *args;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
-  b200_count_launches(1);
-  if (a.elem == ELEM_BF16) act_grad_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
-  else act_grad_kernel<__half><<<grid, 128, 0, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.dbias == nullptr) return static_cast<int>(e);
+  const cudaError_t launched = a.elem == ELEM_BF16 ? act_grad_launch<__nv_bfloat16>(a, st) : act_grad_launch<__half>(a, st);
+  if (launched != cudaSuccess || a.dbias == nullptr) return static_cast<int>(launched);
   b200_count_launches(1);
   const dim3 fin((a.N + 255) / 256, a.G);
+  cudaError_t e;
   if (a.elem == ELEM_BF16) e = launch_chained(bias_grad_kernel<__nv_bfloat16>, fin, dim3(256), 0, st, a);
   else e = launch_chained(bias_grad_kernel<__half>, fin, dim3(256), 0, st, a);
   return static_cast<int>(e);

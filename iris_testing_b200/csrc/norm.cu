@@ -8,10 +8,13 @@
 //   dres = s gh        dgate = sum over what the gate was spread over of gh u
 //   q = gate gh w      dy = r1 (q - yh mean(q yh))        yh = y r1       dw  = sum_rows gate gh yh
 //
-// A row stays in the registers of the threads that share it (a warp up to 32 packs of a row, a block above that),
-// so every tensor is read and written once.  The backward pass computes h again from y and res, which are
-// kept for it anyway, instead of reading the rounded h.  Sums over rows (dw, dw2, dgate of one value per column) are
-// kept per thread over the rows of a block, written once per block and added up in a fixed order by a second kernel.
+// A row stays in the registers of the threads that share it, 16 elements each (a warp up to 512 columns, a block above
+// that), so every tensor is read and written once; blocks are persistent, and the next rows are on their way
+// (cp.async into slots that each thread fills and reads itself) while a row is reduced.  With 8 elements a thread, the
+// reductions were a third of 46 instructions per 32 elements and the kernels bound by issue.  The backward
+// pass computes h again from y and res, which are kept for it anyway, instead of reading the rounded h.  Sums over rows
+// (dw2, and A = sum gh yh, of which dw is gate times and the gradient of a gate per column w times) are kept per thread
+// over the rows of a block, written once per block and added up in a fixed order by a second kernel.
 #include <cuda_runtime.h>
 
 #include "elementwise.cuh"
@@ -37,7 +40,7 @@ typedef struct b200_norm_args {
   void* dgate;            // gate_kind 2: [T], 3: [T, H]; 1: [H], written by the finishing kernel
   void* dw;               // [H] or null
   void* dw2;              // [H] or null
-  float* partial;         // [3][parts][H]: dw, dw2, dgate of each block
+  float* partial;         // [2][parts][H]: A and dw2 of each block
   long long ld_y, ld_res, ld_gate, ld_dh, ld_dn;
   int T, H;
   int elem;               // ElemType of y, res, h, n
@@ -45,7 +48,7 @@ typedef struct b200_norm_args {
   int norm;               // 0: u = y
   int gate_kind;          // 0 none, 1 [H], 2 one per row, 3 [T, H]
   int aligned;            // every row starts on 16 bytes and H is a whole number of packs
-  int parts;              // rows of `partial`
+  int parts;              // rows in work at once (set by the launcher)
   float scale, eps;
 } b200_norm_args;
 }
@@ -53,268 +56,426 @@ typedef struct b200_norm_args {
 namespace b200 {
 
 constexpr int NORM_MAX_H = 16384;
-constexpr int NORM_WARP_ROWS = 4;     // rows of a block where a warp has a row
+constexpr int NORM_WARP_ROWS = 4;      // rows of a block where a warp has a row
+constexpr int NORM_ELEMS = 16;         // elements of a row per thread (8 where that is enough)
 
-template <typename T, int VEC, int VPT, bool WARP_ROW>
-__global__ void __launch_bounds__(WARP_ROW ? NORM_WARP_ROWS * 32 : 1024) norm_forward_kernel(const b200_norm_args a) {
-  __shared__ float slot[2][32];
-  const int row = WARP_ROW ? blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-  const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
-  const int stride = (WARP_ROW ? 32 : blockDim.x) * VEC;
-  if (row >= a.T) return;
-  const T* y = static_cast<const T*>(a.y) + row * a.ld_y;
-  const T* res = static_cast<const T*>(a.res) + (a.res != nullptr ? row * a.ld_res : 0);
-  const size_t out = static_cast<size_t>(row) * a.H;
-  const float inv_h = 1.f / static_cast<float>(a.H);
+// Threads of a block and blocks of an SM of a variant: MAXT is the most threads that share a row (32: a warp).  They set
+// the registers a thread may have: forward 80, backward 128, and 64 where 1024 threads share a row (more
+// than 8192 columns).
+template <bool BACK, int MAXT>
+constexpr int NORM_BLOCKS = MAXT == 32 ? (BACK ? 4 : 6) : MAXT == 256 ? (BACK ? 2 : 3) : 1;
+template <int MAXT>
+constexpr int NORM_THREADS = MAXT == 32 ? NORM_WARP_ROWS * 32 : MAXT;
+// Rows on their way ahead of the one in work: up to three, by the slots that fit beside each other on an SM (two tensors
+// forward, four backward); none for the widest rows and for rows that do not lie on 16 bytes, which go straight to
+// registers.
+template <bool BACK, int VEC, int VPT, int MAXT>
+constexpr int NORM_SLOT_ROW = (BACK ? 4 : 2) * VPT * NORM_THREADS<MAXT> * 16 * NORM_BLOCKS<BACK, MAXT>;
+template <bool BACK, int VEC, int VPT, int MAXT>
+constexpr int NORM_STAGES = VEC == 1 || MAXT == 1024 ? 0
+                            : 3 * NORM_SLOT_ROW<BACK, VEC, VPT, MAXT> <= 200 * 1024 ? 3
+                                                                                    : 200 * 1024 / NORM_SLOT_ROW<BACK, VEC, VPT, MAXT>;
 
-  float u[VPT][VEC], v[VPT][VEC];
-  float ss = 0.f;
+// Asks for every pack that this thread takes of a row.
+template <typename T, int VEC, int VPT>
+__device__ __forceinline__ void fetch_row(const void* base, long long ld, int row, int H, int t, int stride, uint4* slot, int threads) {
+  if (base == nullptr) return;
+  const T* p = static_cast<const T*>(base) + row * ld;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = t * VEC + i * stride;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) u[i][j] = v[i][j] = 0.f;
-    if (c < a.H) {
-      load_pack<T, VEC>(y + c, u[i]);
-      if (a.res != nullptr) load_pack<T, VEC>(res + c, v[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) ss += u[i][j] * u[i][j];
-  }
-  float r1 = 1.f;
-  if (a.norm) {
-    r1 = rsqrtf(row_sum<WARP_ROW>(ss, slot[0]) * inv_h + a.eps);
-    if (a.r1 != nullptr && t == 0) a.r1[row] = r1;
-  }
-  float gate_row = 1.f;
-  if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, reinterpret_cast<float(&)[1]>(gate_row));
-  float ss2 = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = t * VEC + i * stride;
-    if (c >= a.H) continue;
-    float w[VEC], g[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { w[j] = 1.f; g[j] = gate_row; }
-    if (a.w != nullptr) load_param<T, VEC>(a.w, a.w_f32, c, w);
-    if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, g);
-    if (a.gate_kind == 3) load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float uu = u[i][j] * r1 * w[j];
-      u[i][j] = a.res != nullptr ? fmaf(g[j], uu, a.scale * v[i][j]) : uu;
-      ss2 += u[i][j] * u[i][j];
-    }
-    store_pack<T, VEC>(static_cast<T*>(a.h) + out + c, u[i]);
-  }
-  if (a.w2 == nullptr) return;
-  const float r2 = rsqrtf(row_sum<WARP_ROW>(ss2, slot[1]) * inv_h + a.eps);
-  if (a.r2 != nullptr && t == 0) a.r2[row] = r2;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = t * VEC + i * stride;
-    if (c >= a.H) continue;
-    float w[VEC];
-    load_param<T, VEC>(a.w2, a.w2_f32, c, w);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) u[i][j] *= r2 * w[j];
-    store_pack<T, VEC>(static_cast<T*>(a.n) + out + c, u[i]);
+    if (c < H) async_copy_16(slot + i * threads, p + c);
   }
 }
 
-template <typename T, int VEC, int VPT, bool WARP_ROW>
-__global__ void __launch_bounds__(WARP_ROW ? NORM_WARP_ROWS * 32 : 1024) norm_backward_kernel(const b200_norm_args a) {
-  __shared__ float slot[2][3][32];       // two sets: a row's sums while a slow warp still reads the row before's
+// One pack of a tensor: from this thread's slot, or straight from memory where rows are not fetched ahead.
+template <typename T, int VEC, int S>
+__device__ __forceinline__ void read_pack(const uint4* slot, const void* base, long long ld, int row, int c, float (&out)[VEC]) {
+  if constexpr (S > 0) load_pack<T, VEC>(reinterpret_cast<const T*>(slot), out);
+  else load_pack<T, VEC>(static_cast<const T*>(base) + row * ld + c, out);
+}
+
+template <typename T, int VEC, int VPT, int MAXT>
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) norm_forward_kernel(const b200_norm_args a) {
+  extern __shared__ uint4 slots[];
+  __shared__ __align__(16) float sums[2][2][32];       // two sets: a row's sums while a slow warp still reads the row before's
+  constexpr bool WARP_ROW = MAXT == 32;
+  constexpr int S = NORM_STAGES<false, VEC, VPT, MAXT>;
   const int part = WARP_ROW ? blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
   const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
-  const int stride = (WARP_ROW ? 32 : blockDim.x) * VEC;
+  const int threads = blockDim.x, stride = (WARP_ROW ? 32 : threads) * VEC;
   const float inv_h = 1.f / static_cast<float>(a.H);
-  const bool junction = a.res != nullptr;
+  const int tensors = a.res != nullptr ? 2 : 1;
+  uint4* mine = slots + threadIdx.x;                       // [stage][tensor][VPT][threads]
+  auto at = [&](int stage, int tensor) { return mine + (stage * tensors + tensor) * VPT * threads; };
+  auto fetch = [&](int row, int stage) {
+    if constexpr (S > 0) {
+      if (row < a.T) {
+        fetch_row<T, VEC, VPT>(a.y, a.ld_y, row, a.H, t, stride, at(stage, 0), threads);
+        fetch_row<T, VEC, VPT>(a.res, a.ld_res, row, a.H, t, stride, at(stage, 1), threads);
+      }
+      async_commit();
+    }
+  };
+  if constexpr (!WARP_ROW) {
+    if (threadIdx.x < 128) (&sums[0][0][0])[threadIdx.x] = 0.f;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(part + s * a.parts, s);
 
-  float acc_w[VPT][VEC], acc_w2[VPT][VEC], acc_g[VPT][VEC];
+  int set = 0, stage = 0;
+  for (int row = part; row < a.T; row += a.parts, set ^= 1, stage = stage + 1 >= S ? 0 : stage + 1) {
+    if constexpr (S > 0) async_wait<S - 1>();
+    const size_t out = static_cast<size_t>(row) * a.H;
+    float u[VPT][VEC], v[VPT][VEC];
+    float ss[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t * VEC + i * stride;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) u[i][j] = v[i][j] = 0.f;
+      if (c < a.H) {
+        read_pack<T, VEC, S>(at(stage, 0) + i * threads, a.y, a.ld_y, row, c, u[i]);
+        if (a.res != nullptr) read_pack<T, VEC, S>(at(stage, 1) + i * threads, a.res, a.ld_res, row, c, v[i]);
+      }
+      v_dot<VEC>(ss, u[i], u[i]);
+    }
+    float r1 = 1.f;
+    if (a.norm) {
+      r1 = rsqrtf(row_sum<WARP_ROW>(ss[0] + ss[1], sums[set][0]) * inv_h + a.eps);
+      if (a.r1 != nullptr && t == 0) a.r1[row] = r1;
+    }
+    fetch(row + S * a.parts, stage);
+    float gate_row[1] = {1.f};
+    if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, gate_row);
+    ss[0] = ss[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t * VEC + i * stride;
+      if (c >= a.H) continue;
+      float w[VEC];
+      if (a.norm) v_mul<VEC>(u[i], u[i], r1);
+      if (a.w != nullptr) {
+        load_param<T, VEC>(a.w, a.w_f32, c, w);
+        v_mul<VEC>(u[i], u[i], w);
+      }
+      if (a.res != nullptr) {
+        v_mul<VEC>(v[i], v[i], a.scale);
+        if (a.gate_kind == 1 || a.gate_kind == 3) {
+          if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, w);
+          else load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, w);
+          v_fma<VEC>(u[i], u[i], w, v[i]);
+        } else {
+          v_fma<VEC>(u[i], u[i], gate_row[0], v[i]);
+        }
+      }
+      if (a.w2 != nullptr) v_dot<VEC>(ss, u[i], u[i]);
+      store_pack<T, VEC>(static_cast<T*>(a.h) + out + c, u[i]);
+    }
+    if (a.w2 == nullptr) continue;
+    const float r2 = rsqrtf(row_sum<WARP_ROW>(ss[0] + ss[1], sums[set][1]) * inv_h + a.eps);
+    if (a.r2 != nullptr && t == 0) a.r2[row] = r2;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t * VEC + i * stride;
+      if (c >= a.H) continue;
+      float w[VEC];
+      load_param<T, VEC>(a.w2, a.w2_f32, c, w);
+      v_mul<VEC>(u[i], u[i], r2);
+      v_mul<VEC>(u[i], u[i], w);
+      store_pack<T, VEC>(static_cast<T*>(a.n) + out + c, u[i]);
+    }
+  }
+  if constexpr (S > 0) async_wait<0>();
+}
+
+template <typename T, int VEC, int VPT, int MAXT>
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) norm_backward_kernel(const b200_norm_args a) {
+  extern __shared__ uint4 slots[];
+  __shared__ __align__(16) float sums[2][3][32];
+  constexpr bool WARP_ROW = MAXT == 32;
+  constexpr int S = NORM_STAGES<true, VEC, VPT, MAXT>;
+  const int part = WARP_ROW ? blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+  const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
+  const int threads = blockDim.x, stride = (WARP_ROW ? 32 : threads) * VEC;
+  const float inv_h = 1.f / static_cast<float>(a.H);
+  const bool next = a.dn != nullptr;
+  uint4* mine = slots + threadIdx.x;                       // [stage][y, dh, res, dn][VPT][threads]
+  const int tensors = next ? 4 : 2;
+  auto at = [&](int stage, int tensor) { return mine + (stage * tensors + tensor) * VPT * threads; };
+  auto fetch = [&](int row, int stage) {
+    if constexpr (S > 0) {
+      if (row < a.T) {
+        fetch_row<T, VEC, VPT>(a.y, a.ld_y, row, a.H, t, stride, at(stage, 0), threads);
+        fetch_row<T, VEC, VPT>(a.dh, a.ld_dh, row, a.H, t, stride, at(stage, 1), threads);
+        if (next) {
+          fetch_row<T, VEC, VPT>(a.res, a.ld_res, row, a.H, t, stride, at(stage, 2), threads);
+          fetch_row<T, VEC, VPT>(a.dn, a.ld_dn, row, a.H, t, stride, at(stage, 3), threads);
+        }
+      }
+      async_commit();
+    }
+  };
+  if constexpr (!WARP_ROW) {
+    for (int i = threadIdx.x; i < 192; i += threads) (&sums[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(part + s * a.parts, s);
+
+  float acc[VPT][VEC], acc2[VPT][VEC];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc_w[i][j] = acc_w2[i][j] = acc_g[i][j] = 0.f;
+    for (int j = 0; j < VEC; ++j) acc[i][j] = acc2[i][j] = 0.f;
 
-  int set = 0;
-  for (int row = part; row < a.T; row += a.parts, set ^= 1) {
+  int set = 0, stage = 0;
+  for (int row = part; row < a.T; row += a.parts, set ^= 1, stage = stage + 1 >= S ? 0 : stage + 1) {
+    if constexpr (S > 0) async_wait<S - 1>();
     const float r1 = a.norm ? a.r1[row] : 1.f;
-    const float r2 = a.dn != nullptr ? a.r2[row] : 0.f;
-    float gate_row = 1.f;
-    if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, reinterpret_cast<float(&)[1]>(gate_row));
+    const float r2 = next ? a.r2[row] : 0.f;
+    float gate_row[1] = {1.f};
+    if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, gate_row);
+    // x *= the gate's values of a pack
+    auto times_gate = [&](int c, float (&x)[VEC]) {
+      if (a.gate_kind == 0) return;
+      if (a.gate_kind == 2) {
+        v_mul<VEC>(x, x, gate_row[0]);
+        return;
+      }
+      float g[VEC];
+      if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, g);
+      else load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
+      v_mul<VEC>(x, x, g);
+    };
+    auto times_weight = [&](int c, float (&x)[VEC]) {
+      if (a.w == nullptr) return;
+      float w[VEC];
+      load_param<T, VEC>(a.w, a.w_f32, c, w);
+      v_mul<VEC>(x, x, w);
+    };
     float yh[VPT][VEC], hh[VPT][VEC], gh[VPT][VEC];
-    float m = 0.f;
+    float m[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t * VEC + i * stride;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) yh[i][j] = hh[i][j] = gh[i][j] = 0.f;
       if (c >= a.H) continue;
-      load_pack<T, VEC>(static_cast<const T*>(a.y) + row * a.ld_y + c, yh[i]);
+      read_pack<T, VEC, S>(at(stage, 0) + i * threads, a.y, a.ld_y, row, c, yh[i]);
+      if (a.norm) v_mul<VEC>(yh[i], yh[i], r1);
+      if (next) {
+        float x[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) yh[i][j] *= r1;
-      if (a.dn != nullptr) {
-        float res[VEC], w[VEC], g[VEC], dn[VEC], w2[VEC];
-        load_pack<T, VEC>(static_cast<const T*>(a.res) + row * a.ld_res + c, res);
-        load_pack<T, VEC>(static_cast<const T*>(a.dn) + row * a.ld_dn + c, dn);
-        load_param<T, VEC>(a.w2, a.w2_f32, c, w2);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { w[j] = 1.f; g[j] = gate_row; }
-        if (a.w != nullptr) load_param<T, VEC>(a.w, a.w_f32, c, w);
-        if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, g);
-        if (a.gate_kind == 3) load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          hh[i][j] = fmaf(g[j], yh[i][j] * w[j], a.scale * res[j]) * r2;
-          acc_w2[i][j] += dn[j] * hh[i][j];
-          gh[i][j] = dn[j] * w2[j];
-          m += gh[i][j] * hh[i][j];
-        }
+        for (int j = 0; j < VEC; ++j) x[j] = yh[i][j];
+        times_weight(c, x);
+        times_gate(c, x);
+        read_pack<T, VEC, S>(at(stage, 2) + i * threads, a.res, a.ld_res, row, c, hh[i]);
+        v_fma<VEC>(hh[i], hh[i], a.scale, x);
+        v_mul<VEC>(hh[i], hh[i], r2);
+        read_pack<T, VEC, S>(at(stage, 3) + i * threads, a.dn, a.ld_dn, row, c, gh[i]);
+        v_fma<VEC>(acc2[i], gh[i], hh[i], acc2[i]);
+        load_param<T, VEC>(a.w2, a.w2_f32, c, x);
+        v_mul<VEC>(gh[i], gh[i], x);
+        v_dot<VEC>(m, gh[i], hh[i]);
       }
     }
-    if (a.dn != nullptr) m = row_sum<WARP_ROW>(m, slot[set][0]) * inv_h;
-    float mq = 0.f, mg = 0.f;
+    const float mean = next ? row_sum<WARP_ROW>(m[0] + m[1], sums[set][0]) * inv_h : 0.f;
+    float mq[2] = {0.f, 0.f}, mg[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t * VEC + i * stride;
       if (c >= a.H) continue;
-      float w[VEC], g[VEC], d[VEC], p[VEC];
+      float d[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) { w[j] = 1.f; g[j] = gate_row; d[j] = 0.f; }
-      if (a.dh != nullptr) load_pack<T, VEC>(static_cast<const T*>(a.dh) + row * a.ld_dh + c, d);
-      if (a.w != nullptr) load_param<T, VEC>(a.w, a.w_f32, c, w);
-      if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, g);
-      if (a.gate_kind == 3) load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (a.dn != nullptr) d[j] += r2 * (gh[i][j] - hh[i][j] * m);
-        p[j] = d[j] * yh[i][j] * w[j];          // d(gate)
-        mg += p[j];
-        acc_g[i][j] += p[j];
-        const float du = g[j] * d[j];
-        acc_w[i][j] += du * yh[i][j];
-        gh[i][j] = du * w[j];                   // q
-        mq += gh[i][j] * yh[i][j];
-        d[j] *= a.scale;
+      for (int j = 0; j < VEC; ++j) d[j] = 0.f;
+      if (a.dh != nullptr) read_pack<T, VEC, S>(at(stage, 1) + i * threads, a.dh, a.ld_dh, row, c, d);
+      if (next) {
+        v_fma<VEC>(gh[i], hh[i], -mean, gh[i]);
+        v_fma<VEC>(d, gh[i], r2, d);
       }
-      if (a.dres != nullptr) store_pack<T, VEC>(static_cast<T*>(a.dres) + static_cast<size_t>(row) * a.H + c, d);
-      if (junction && a.gate_kind == 3 && a.dgate != nullptr)
-        store_pack<T, VEC>(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * a.H + c, p);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) gh[i][j] = d[j];
+      if (a.gate_kind >= 2) {                     // a gate that changes from row to row: its own gradient, and A takes it in
+        float p[VEC];
+        v_mul<VEC>(p, d, yh[i]);
+        times_weight(c, p);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mg[j & 1] += p[j];
+        if (a.gate_kind == 3 && a.dgate != nullptr) store_pack<T, VEC>(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * a.H + c, p);
+        times_gate(c, gh[i]);
+        v_fma<VEC>(acc[i], gh[i], yh[i], acc[i]);
+      } else {
+        v_fma<VEC>(acc[i], gh[i], yh[i], acc[i]);
+        times_gate(c, gh[i]);
+      }
+      times_weight(c, gh[i]);                     // q
+      v_dot<VEC>(mq, gh[i], yh[i]);
+      if (a.dres != nullptr) {
+        v_mul<VEC>(d, d, a.scale);
+        store_pack<T, VEC>(static_cast<T*>(a.dres) + static_cast<size_t>(row) * a.H + c, d);
+      }
     }
+    fetch(row + S * a.parts, stage);
     if (a.gate_kind == 2 && a.dgate != nullptr) {
-      mg = row_sum<WARP_ROW>(mg, slot[set][1]);
+      const float g = row_sum<WARP_ROW>(mg[0] + mg[1], sums[set][1]);
       if (t == 0) {
-        if (a.gate_f32) static_cast<float*>(a.dgate)[row] = mg;
-        else static_cast<T*>(a.dgate)[row] = from_f32<T>(mg);
+        if (a.gate_f32) static_cast<float*>(a.dgate)[row] = g;
+        else static_cast<T*>(a.dgate)[row] = from_f32<T>(g);
       }
     }
-    if (a.norm) mq = row_sum<WARP_ROW>(mq, slot[set][2]) * inv_h;
+    const float mean_q = a.norm ? row_sum<WARP_ROW>(mq[0] + mq[1], sums[set][2]) * inv_h : 0.f;
     if (a.dy != nullptr) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = t * VEC + i * stride;
         if (c >= a.H) continue;
-        float d[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) d[j] = a.norm ? r1 * (gh[i][j] - yh[i][j] * mq) : gh[i][j];
-        store_pack<T, VEC>(static_cast<T*>(a.dy) + static_cast<size_t>(row) * a.H + c, d);
+        if (a.norm) {
+          v_fma<VEC>(gh[i], yh[i], -mean_q, gh[i]);
+          v_mul<VEC>(gh[i], gh[i], r1);
+        }
+        store_pack<T, VEC>(static_cast<T*>(a.dy) + static_cast<size_t>(row) * a.H + c, gh[i]);
       }
     }
   }
-  const size_t plane = static_cast<size_t>(a.parts) * a.H, at = static_cast<size_t>(part) * a.H;
+  if constexpr (S > 0) async_wait<0>();
+  if (a.partial == nullptr) return;
+  const size_t plane = static_cast<size_t>(a.parts) * a.H, here = static_cast<size_t>(part) * a.H;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = t * VEC + i * stride;
     if (c >= a.H) continue;
+    constexpr int Q = VEC < 4 ? VEC : 4;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (a.dw != nullptr) a.partial[at + c + j] = acc_w[i][j];
-      if (a.dw2 != nullptr) a.partial[plane + at + c + j] = acc_w2[i][j];
-      if (a.gate_kind == 1 && a.dgate != nullptr) a.partial[2 * plane + at + c + j] = acc_g[i][j];
+    for (int q = 0; q < VEC; q += Q) {
+      store_pack<float, Q>(a.partial + here + c + q, reinterpret_cast<float(&)[Q]>(acc[i][q]));
+      if (a.dw2 != nullptr) store_pack<float, Q>(a.partial + plane + here + c + q, reinterpret_cast<float(&)[Q]>(acc2[i][q]));
     }
   }
 }
 
-// out[c] = sum over the parts of partial[.][c], in their order within each of eight interleaved shares.
+// Column sums over the parts, in their order within each of 32 interleaved shares: dw = gate A, the gate's w A, and dw2.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_columns_kernel(const b200_norm_args a) {
-  __shared__ float share[8][33];
+__global__ void __launch_bounds__(1024) norm_columns_kernel(const b200_norm_args a) {
+  __shared__ float share[32][33];
   chain_wait();
-  const int which = blockIdx.y;
-  void* out = which == 0 ? a.dw : which == 1 ? a.dw2 : (a.gate_kind == 1 ? a.dgate : nullptr);
-  if (out == nullptr) return;
-  const int f32 = which == 0 ? a.w_f32 : which == 1 ? a.w2_f32 : a.gate_f32;
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), s = threadIdx.x >> 5;
-  const float* p = a.partial + static_cast<size_t>(which) * a.parts * a.H;
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  if (blockIdx.y == 1 ? a.dw2 == nullptr : a.dw == nullptr && a.dgate == nullptr) return;
+  const float* p = a.partial + static_cast<size_t>(blockIdx.y) * a.parts * a.H;
   float v = 0.f;
-  if (c < a.H)
-    for (int k = s; k < a.parts; k += 8) v += p[static_cast<size_t>(k) * a.H + c];
-  share[s][threadIdx.x & 31] = v;
+  if (c < a.H) {
+#pragma unroll 4
+    for (int k = s; k < a.parts; k += 32) v += p[static_cast<size_t>(k) * a.H + c];
+  }
+  share[s][lane] = v;
   __syncthreads();
-  if (s == 0 && c < a.H) {
+  if (s != 0 || c >= a.H) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) v += share[k][threadIdx.x];
-    if (f32) static_cast<float*>(out)[c] = v;
-    else static_cast<T*>(out)[c] = from_f32<T>(v);
+  for (int k = 1; k < 32; ++k) v += share[k][lane];
+  auto put = [&](void* out, int f32, float x) {
+    if (f32) static_cast<float*>(out)[c] = x;
+    else static_cast<T*>(out)[c] = from_f32<T>(x);
+  };
+  if (blockIdx.y == 1) {
+    put(a.dw2, a.w2_f32, v);
+    return;
   }
+  float w[1] = {1.f}, g[1] = {1.f};
+  if (a.w != nullptr) load_param<T, 1>(a.w, a.w_f32, c, w);
+  if (a.gate_kind == 1) load_param<T, 1>(a.gate, a.gate_f32, c, g);
+  if (a.dw != nullptr) put(a.dw, a.w_f32, g[0] * v);
+  if (a.gate_kind == 1 && a.dgate != nullptr) put(a.dgate, a.gate_f32, w[0] * v);
 }
 
-// How a row is shared: packs of VEC elements, VPT of them per thread, `threads` threads (32: a warp per row).
-struct NormShape {
-  int threads, vpt;
-};
-static NormShape norm_shape(int H, int vec) {
+// How a row is shared: a warp while 16 elements a lane are enough, which needs no barrier, otherwise the threads of a block.
+template <int MAXT>
+static int norm_row_threads(int H, int vec, int vpt) {
   const int packs = (H + vec - 1) / vec;
-  const int vpt = vec > 1 ? (packs <= 32 ? 1 : packs <= 1024 ? 2 : 4) : (packs <= 1024 ? 4 : 16);
-  int threads = ((packs + vpt - 1) / vpt + 31) / 32 * 32;
-  return {threads, vpt};
+  return MAXT == 32 ? 32 : ((packs + vpt - 1) / vpt + 31) / 32 * 32;
 }
 
-static int norm_vec(const b200_norm_args& a) { return a.aligned ? (a.elem == ELEM_F32 ? 4 : 8) : 1; }
+// Rows (of warps, or of blocks) in work at once: the blocks that the registers of the variant and the slots leave room
+// for on every SM, and no more rows than there are.
+template <bool BACK, int MAXT>
+static int norm_parts(int T, int threads, size_t smem, int sms) {
+  const int rows = MAXT == 32 ? NORM_WARP_ROWS : 1;
+  int per_sm = MAXT == 32 ? NORM_BLOCKS<BACK, 32> : MAXT * NORM_BLOCKS<BACK, MAXT> / threads;
+  const int fit = static_cast<int>((224u * 1024u) / (smem + 2048));      // beside 1 KB of the system's and the sums
+  if (fit < per_sm) per_sm = fit > 0 ? fit : 1;
+  const int blocks = (T + rows - 1) / rows;
+  return rows * (blocks < per_sm * sms ? blocks : per_sm * sms);
+}
 
-template <bool BACK, typename T, int VEC, int VPT>
-static cudaError_t norm_launch(const b200_norm_args& a, int threads, cudaStream_t st) {
-  const bool warp_row = threads <= 32;
-  b200_count_launches(1);
-  if constexpr (!BACK) {
-    if (warp_row) norm_forward_kernel<T, VEC, VPT, true><<<(a.T + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS, NORM_WARP_ROWS * 32, 0, st>>>(a);
-    else norm_forward_kernel<T, VEC, VPT, false><<<a.T, threads, 0, st>>>(a);
-    return cudaGetLastError();
-  } else {
-    if (warp_row) norm_backward_kernel<T, VEC, VPT, true><<<a.parts / NORM_WARP_ROWS, NORM_WARP_ROWS * 32, 0, st>>>(a);
-    else norm_backward_kernel<T, VEC, VPT, false><<<a.parts, threads, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || (a.dw == nullptr && a.dw2 == nullptr && !(a.gate_kind == 1 && a.dgate != nullptr))) return e;
-    b200_count_launches(1);
-    return launch_chained(norm_columns_kernel<T>, dim3((a.H + 31) / 32, 3), dim3(256), 0, st, a);
+template <bool BACK, typename T, int VEC, int VPT, int MAXT>
+static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
+  const int threads = norm_row_threads<MAXT>(a.H, VEC, VPT);
+  const int block = MAXT == 32 ? NORM_WARP_ROWS * 32 : threads;
+  const int tensors = BACK ? (a.dn != nullptr ? 4 : 2) : (a.res != nullptr ? 2 : 1);
+  const size_t smem = static_cast<size_t>(NORM_STAGES<BACK, VEC, VPT, MAXT>) * tensors * VPT * block * 16;      // at most 192 KB
+  a.parts = norm_parts<BACK, MAXT>(a.T, threads, smem, sms);
+  const dim3 grid(MAXT == 32 ? a.parts / NORM_WARP_ROWS : a.parts);
+  auto kern = BACK ? norm_backward_kernel<T, VEC, VPT, MAXT> : norm_forward_kernel<T, VEC, VPT, MAXT>;
+  if (smem > 40 * 1024) {          // 48 KB, static shared memory included, need no leave
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
   }
+  b200_count_launches(1);
+  kern<<<grid, block, smem, st>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (!BACK || e != cudaSuccess || a.partial == nullptr) return e;
+  b200_count_launches(1);
+  return launch_chained(norm_columns_kernel<T>, dim3((a.H + 31) / 32, a.dw2 != nullptr ? 2 : 1), dim3(1024), 0, st, a);
+}
+
+// Calls f<VEC, VPT, MAXT> for rows of H elements.
+template <typename T, typename F>
+static auto norm_variant(int H, bool aligned, F&& f) {
+  constexpr int V = 16 / sizeof(T);
+  if (!aligned) {
+    if (H <= 32 * NORM_ELEMS) return f.template operator()<1, NORM_ELEMS, 32>();
+    if (H <= 256 * NORM_ELEMS) return f.template operator()<1, NORM_ELEMS, 256>();
+    return f.template operator()<1, NORM_ELEMS, 1024>();
+  }
+  if (H <= 256) return f.template operator()<V, 8 / V, 32>();
+  if (H <= 32 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 32>();
+  if (H <= 256 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 256>();
+  if (H <= 512 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 512>();
+  return f.template operator()<V, NORM_ELEMS / V, 1024>();
 }
 
 template <bool BACK, typename T>
-static cudaError_t norm_dispatch(const b200_norm_args& a, cudaStream_t st) {
-  constexpr int VEC = 16 / sizeof(T);
-  const NormShape s = norm_shape(a.H, a.aligned ? VEC : 1);
-  if (a.aligned) {
-    if (s.vpt == 1) return norm_launch<BACK, T, VEC, 1>(a, s.threads, st);
-    if (s.vpt == 2) return norm_launch<BACK, T, VEC, 2>(a, s.threads, st);
-    return norm_launch<BACK, T, VEC, 4>(a, s.threads, st);
-  }
-  if (s.vpt == 4) return norm_launch<BACK, T, 1, 4>(a, s.threads, st);
-  return norm_launch<BACK, T, 1, 16>(a, s.threads, st);
+struct NormLaunch {
+  const b200_norm_args& a;
+  int sms;
+  cudaStream_t st;
+  template <int VEC, int VPT, int MAXT>
+  int operator()() const { return static_cast<int>(norm_launch<BACK, T, VEC, VPT, MAXT>(a, sms, st)); }
+};
+template <typename T>
+static int norm_dispatch(bool back, const b200_norm_args& a, int sms, cudaStream_t st) {
+  return back ? norm_variant<T>(a.H, a.aligned != 0, NormLaunch<true, T>{a, sms, st})
+              : norm_variant<T>(a.H, a.aligned != 0, NormLaunch<false, T>{a, sms, st});
 }
 
+// The most rows that a backward pass has in work at once.
+struct NormPartsOf {
+  int T, H, sms;
+  template <int VEC, int VPT, int MAXT>
+  int operator()() const { return norm_parts<true, MAXT>(T, norm_row_threads<MAXT>(H, VEC, VPT), 0, sms); }
+};
+
 template <bool BACK>
-static int norm_run(const b200_norm_args* a, void* stream) {
-  if (a == nullptr || a->T < 1 || a->H < 1 || a->H > NORM_MAX_H || a->y == nullptr || a->gate_kind < 0 || a->gate_kind > 3) return -10;
+static int norm_run(const b200_norm_args* a, int sms, void* stream) {
+  if (a == nullptr || sms < 1 || a->T < 1 || a->H < 1 || a->H > NORM_MAX_H || a->y == nullptr || a->gate_kind < 0 || a->gate_kind > 3) return -10;
   if ((a->gate_kind != 0 && (a->gate == nullptr || a->res == nullptr)) || (a->w2 != nullptr && a->res == nullptr)) return -11;
   if (!BACK && (a->h == nullptr || (a->w2 != nullptr && a->n == nullptr))) return -12;
-  if (BACK && (a->parts < 1 || (a->norm && a->r1 == nullptr) || (a->dn != nullptr && (a->r2 == nullptr || a->w2 == nullptr)))) return -13;
+  if (BACK && ((a->norm && a->r1 == nullptr) || (a->dn != nullptr && (a->r2 == nullptr || a->w2 == nullptr)))) return -13;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a->elem) {
-    case ELEM_F32: return static_cast<int>(norm_dispatch<BACK, float>(*a, st));
-    case ELEM_BF16: return static_cast<int>(norm_dispatch<BACK, __nv_bfloat16>(*a, st));
-    case ELEM_F16: return static_cast<int>(norm_dispatch<BACK, __half>(*a, st));
+    case ELEM_F32: return norm_dispatch<float>(BACK, *a, sms, st);
+    case ELEM_BF16: return norm_dispatch<__nv_bfloat16>(BACK, *a, sms, st);
+    case ELEM_F16: return norm_dispatch<__half>(BACK, *a, sms, st);
   }
   return -14;
 }
@@ -323,19 +484,14 @@ static int norm_run(const b200_norm_args* a, void* stream) {
 
 extern "C" {
 
-int b200_norm_forward(const b200_norm_args* a, void* stream) { return b200::norm_run<false>(a, stream); }
-int b200_norm_backward(const b200_norm_args* a, void* stream) { return b200::norm_run<true>(a, stream); }
+int b200_norm_forward(const b200_norm_args* a, int sms, void* stream) { return b200::norm_run<false>(a, sms, stream); }
+// `partial` has 2 * b200_norm_parts() * H floats where dw, dw2 or the gradient of a gate per column is asked for.
+int b200_norm_backward(const b200_norm_args* a, int sms, void* stream) { return b200::norm_run<true>(a, sms, stream); }
 
-// Rows of `partial` that a backward call of this shape uses: one per block, or per warp where a warp has a row.
 int b200_norm_parts(int T, int H, int elem, int aligned, int sms) {
   using namespace b200;
-  const NormShape s = norm_shape(H, aligned ? (elem == ELEM_F32 ? 4 : 8) : 1);
-  if (s.threads <= 32) {
-    const int blocks = (T + NORM_WARP_ROWS - 1) / NORM_WARP_ROWS;
-    return NORM_WARP_ROWS * (blocks < 4 * sms ? blocks : 4 * sms);
-  }
-  const int per_sm = s.threads <= 128 ? 4 : s.threads <= 256 ? 2 : 1;
-  return T < per_sm * sms ? T : per_sm * sms;
+  const NormPartsOf f{T, H, sms};
+  return elem == ELEM_F32 ? norm_variant<float>(H, aligned != 0, f) : norm_variant<__half>(H, aligned != 0, f);
 }
 
 int b200_abi_size_norm_args() { return static_cast<int>(sizeof(b200_norm_args)); }

@@ -20,7 +20,7 @@ MAX_BALANCE_EXPERTS = 1024
 
 class BalanceArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("logits", "idx", "seq_rows", "mask", "loss", "counts", "kept", "record", "seq_loss",
-                                          "seq_tokens", "total", "ticket", "grad_loss", "grad", "status")] \
+                                          "seq_z", "seq_tokens", "total", "ticket", "grad_loss", "grad", "status")] \
         + [("ld", C.c_longlong)] + [(n, C.c_int) for n in ("T", "E", "k", "S", "elem", "runs", "run_tokens")] \
         + [("coef", C.c_float), ("z", C.c_float)]
 
@@ -32,7 +32,7 @@ def _fill(logits, k, seq_rows, mask, coef, z, S):
     a.logits, a.ld = logits.data_ptr(), logits.stride(0)
     a.seq_rows = None if seq_rows is None else seq_rows.data_ptr()
     a.mask = None if mask is None else mask.data_ptr()
-    runs = declare("b200_balance_runs", [C.c_int] * 3)(a.T, a.E, sm_count(logits.device))
+    runs = declare("b200_balance_runs", [C.c_int] * 4)(a.T, a.E, a.elem, sm_count(logits.device))
     a.run_tokens = -(-a.T // runs)
     a.runs = -(-a.T // a.run_tokens)
     if seq_rows is not None:
@@ -57,11 +57,13 @@ def _forward(logits, idx, seq_rows, mask, coef, z):
         return loss.zero_(), counts.zero_(), None
     a = _fill(logits, idx.shape[1], seq_rows, mask, coef, z, S)
     keep = torch.empty(S * E + S + 2, dtype=torch.int32, device=dev)          # counts, tokens per sequence, two fp32 words
-    work = torch.empty((a.runs + S) * (2 * E + 2) + 2 * S + 1, dtype=torch.float32, device=dev)
+    parts = S * -(-E // 32)
+    work = torch.empty((a.runs + S) * (2 * E + 2) + parts + S + 1, dtype=torch.float32, device=dev)
     a.idx, a.loss, a.counts = idx.data_ptr(), loss.data_ptr(), counts.data_ptr()
     a.record = work.data_ptr()
     a.seq_loss = a.record + 4 * (a.runs + S) * (2 * E + 2)
-    a.ticket = a.seq_loss + 8 * S
+    a.seq_z = a.seq_loss + 4 * parts
+    a.ticket = a.seq_z + 4 * S
     _keep(a, keep, S, E)
     _call("b200_balance_forward", a, logits)
     return loss, counts, keep

@@ -51,6 +51,7 @@ def _check(y, residual, weight, gate, next_weight):
     if not use_native(y):
         return kind
     require(H <= MAX_COLUMNS, f"at most {MAX_COLUMNS} columns (got {H})")
+    require(y.numel() // H <= 2 ** 30, "too many rows")
     require_elem(y, "y")
     require(residual is None or residual.dtype == y.dtype, "residual must have y's dtype")
     for name, w in (("weight", weight), ("next_weight", next_weight), ("gate", gate if kind != GATE_FULL else None)):
@@ -103,9 +104,9 @@ def _align(a: NormArgs, size: int) -> None:
 
 
 def _call(name, a, t):
-    fn = declare(name, [C.POINTER(NormArgs), C.c_void_p])
+    fn = declare(name, [C.POINTER(NormArgs), C.c_int, C.c_void_p])
     with on_device(t):
-        nv.check(fn(C.byref(a), stream_ptr(t)), name.replace("b200_", "").replace("_", " ") + " launch")
+        nv.check(fn(C.byref(a), sm_count(t.device), stream_ptr(t)), name.replace("b200_", "").replace("_", " ") + " launch")
 
 
 def _forward(y, residual, weight, gate, kind, norm, scale, next_weight, eps, save):
@@ -149,10 +150,9 @@ def _backward(saved, kind, norm, scale, eps, need, dh, dn):
     a.r1 = stats.data_ptr()
     a.r2 = a.r1 + 4 * T
     _align(a, y.element_size())
-    parts = declare("b200_norm_parts", [C.c_int] * 5)
-    a.parts = parts(T, a.H, a.elem, a.aligned, sm_count(y.device))
     if a.dw or a.dw2 or (a.dgate and kind == GATE_CHANNEL):
-        partial = torch.empty((3, a.parts, a.H), dtype=torch.float32, device=y.device)
+        parts = declare("b200_norm_parts", [C.c_int] * 5)(T, a.H, a.elem, a.aligned, sm_count(y.device))
+        partial = torch.empty((2, parts, a.H), dtype=torch.float32, device=y.device)
         a.partial = partial.data_ptr()
     _call("b200_norm_backward", a, y)
     return grads
