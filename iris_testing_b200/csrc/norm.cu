@@ -59,22 +59,22 @@ constexpr int NORM_MAX_H = 16384;
 constexpr int NORM_WARP_ROWS = 4;      // rows of a block where a warp has a row
 constexpr int NORM_ELEMS = 16;         // elements of a row per thread (8 where that is enough)
 
-// Threads of a block and blocks of an SM of a variant: MAXT is the most threads that share a row (32: a warp).  They set
-// the registers a thread may have: forward 80, backward 128, and 64 where 1024 threads share a row (more
-// than 8192 columns).
-template <bool BACK, int MAXT>
-constexpr int NORM_BLOCKS = MAXT == 32 ? (BACK ? 4 : 6) : MAXT == 256 ? (BACK ? 2 : 3) : 1;
+// Threads of a block and blocks of an SM of a variant: MAXT is the most threads that share a row (32: a warp).  512
+// threads an SM leave 128 registers each; where 1024 threads share a row (more than 8192 columns) it is 64.
+template <int MAXT>
+constexpr int NORM_BLOCKS = MAXT == 32 ? 4 : MAXT == 256 ? 2 : 1;
 template <int MAXT>
 constexpr int NORM_THREADS = MAXT == 32 ? NORM_WARP_ROWS * 32 : MAXT;
 // Rows on their way ahead of the one in work: up to three, by the slots that fit beside each other on an SM (two tensors
-// forward, four backward); none for the widest rows and for rows that do not lie on 16 bytes, which go straight to
-// registers.
+// forward, four and the two column vectors backward); none for the widest rows and for rows that do not lie on 16 bytes,
+// which go straight to registers.
+constexpr int NORM_SLOT_BYTES = 200 * 1024;
 template <bool BACK, int VEC, int VPT, int MAXT>
-constexpr int NORM_SLOT_ROW = (BACK ? 4 : 2) * VPT * NORM_THREADS<MAXT> * 16 * NORM_BLOCKS<BACK, MAXT>;
+constexpr int NORM_VECTOR_BYTES = BACK && VEC > 1 && MAXT != 1024 ? 2 * VPT * VEC * 4 * NORM_THREADS<MAXT> : 0;
 template <bool BACK, int VEC, int VPT, int MAXT>
-constexpr int NORM_STAGES = VEC == 1 || MAXT == 1024 ? 0
-                            : 3 * NORM_SLOT_ROW<BACK, VEC, VPT, MAXT> <= 200 * 1024 ? 3
-                                                                                    : 200 * 1024 / NORM_SLOT_ROW<BACK, VEC, VPT, MAXT>;
+constexpr int NORM_FIT = (NORM_SLOT_BYTES / NORM_BLOCKS<MAXT> - NORM_VECTOR_BYTES<BACK, VEC, VPT, MAXT>) / ((BACK ? 4 : 2) * VPT * 16 * NORM_THREADS<MAXT>);
+template <bool BACK, int VEC, int VPT, int MAXT>
+constexpr int NORM_STAGES = VEC == 1 || MAXT == 1024 ? 0 : NORM_FIT<BACK, VEC, VPT, MAXT> < 3 ? NORM_FIT<BACK, VEC, VPT, MAXT> : 3;
 
 // Asks for every pack that this thread takes of a row.
 template <typename T, int VEC, int VPT>
@@ -95,8 +95,28 @@ __device__ __forceinline__ void read_pack(const uint4* slot, const void* base, l
   else load_pack<T, VEC>(static_cast<const T*>(base) + row * ld + c, out);
 }
 
+// What a pack's values of norm(y) are multiplied with in every row: w, times the gate where that has a value per column.
+template <typename T, int VEC>
+__device__ __forceinline__ void column_factor(const b200_norm_args& a, int c, float (&f)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) f[j] = 1.f;
+  if (a.w != nullptr) load_param<T, VEC>(a.w, a.w_f32, c, f);
+  if (a.gate_kind == 1) {
+    float g[VEC];
+    load_param<T, VEC>(a.gate, a.gate_f32, c, g);
+    v_mul<VEC>(f, f, g);
+  }
+}
+// What a row is multiplied with: the gate where that has a value per row.
+template <typename T>
+__device__ __forceinline__ float row_factor(const b200_norm_args& a, int row) {
+  float g[1] = {1.f};
+  if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, g);
+  return g[0];
+}
+
 template <typename T, int VEC, int VPT, int MAXT>
-__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) norm_forward_kernel(const b200_norm_args a) {
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_forward_kernel(const b200_norm_args a) {
   extern __shared__ uint4 slots[];
   __shared__ __align__(16) float sums[2][2][32];       // two sets: a row's sums while a slow warp still reads the row before's
   constexpr bool WARP_ROW = MAXT == 32;
@@ -117,17 +137,31 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) 
       async_commit();
     }
   };
-  if constexpr (!WARP_ROW) {
-    if (threadIdx.x < 128) (&sums[0][0][0])[threadIdx.x] = 0.f;
-    __syncthreads();
-  }
 #pragma unroll
   for (int s = 0; s < S; ++s) fetch(part + s * a.parts, s);
+  if constexpr (!WARP_ROW) {
+    if (threadIdx.x < 128) (&sums[0][0][0])[threadIdx.x] = 0.f;
+    for (int i = threadIdx.x + threads; i < 128; i += threads) (&sums[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
+  // the columns' factors stay in registers (of the widest rows they are read again for every row)
+  constexpr bool HELD = MAXT != 1024;
+  float f1[HELD ? VPT : 1][VEC], f2[HELD ? VPT : 1][VEC];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t * VEC + i * stride;
+      if (c >= a.H) continue;
+      column_factor<T, VEC>(a, c, f1[i]);
+      if (a.w2 != nullptr) load_param<T, VEC>(a.w2, a.w2_f32, c, f2[i]);
+    }
+  }
 
   int set = 0, stage = 0;
   for (int row = part; row < a.T; row += a.parts, set ^= 1, stage = stage + 1 >= S ? 0 : stage + 1) {
     if constexpr (S > 0) async_wait<S - 1>();
     const size_t out = static_cast<size_t>(row) * a.H;
+    float r1 = row_factor<T>(a, row);
     float u[VPT][VEC], v[VPT][VEC];
     float ss[2] = {0.f, 0.f};
 #pragma unroll
@@ -141,35 +175,28 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) 
       }
       v_dot<VEC>(ss, u[i], u[i]);
     }
-    float r1 = 1.f;
     if (a.norm) {
-      r1 = rsqrtf(row_sum<WARP_ROW>(ss[0] + ss[1], sums[set][0]) * inv_h + a.eps);
-      if (a.r1 != nullptr && t == 0) a.r1[row] = r1;
+      const float r = rsqrtf(row_sum<WARP_ROW>(ss[0] + ss[1], sums[set][0]) * inv_h + a.eps);
+      if (a.r1 != nullptr && t == 0) a.r1[row] = r;
+      r1 *= r;
     }
     fetch(row + S * a.parts, stage);
-    float gate_row[1] = {1.f};
-    if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, gate_row);
     ss[0] = ss[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t * VEC + i * stride;
       if (c >= a.H) continue;
-      float w[VEC];
-      if (a.norm) v_mul<VEC>(u[i], u[i], r1);
-      if (a.w != nullptr) {
-        load_param<T, VEC>(a.w, a.w_f32, c, w);
-        v_mul<VEC>(u[i], u[i], w);
+      float x[VEC];
+      if constexpr (!HELD) column_factor<T, VEC>(a, c, x);
+      float(&f)[VEC] = HELD ? f1[HELD ? i : 0] : x;
+      v_mul<VEC>(u[i], u[i], r1);
+      if (a.gate_kind == 3) {
+        float g[VEC];
+        load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
+        v_mul<VEC>(u[i], u[i], g);
       }
-      if (a.res != nullptr) {
-        v_mul<VEC>(v[i], v[i], a.scale);
-        if (a.gate_kind == 1 || a.gate_kind == 3) {
-          if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, w);
-          else load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, w);
-          v_fma<VEC>(u[i], u[i], w, v[i]);
-        } else {
-          v_fma<VEC>(u[i], u[i], gate_row[0], v[i]);
-        }
-      }
+      v_mul<VEC>(v[i], v[i], a.scale);              // zeros without a residual
+      v_fma<VEC>(u[i], u[i], f, v[i]);
       if (a.w2 != nullptr) v_dot<VEC>(ss, u[i], u[i]);
       store_pack<T, VEC>(static_cast<T*>(a.h) + out + c, u[i]);
     }
@@ -180,10 +207,11 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) 
     for (int i = 0; i < VPT; ++i) {
       const int c = t * VEC + i * stride;
       if (c >= a.H) continue;
-      float w[VEC];
-      load_param<T, VEC>(a.w2, a.w2_f32, c, w);
+      float x[VEC];
+      if constexpr (!HELD) load_param<T, VEC>(a.w2, a.w2_f32, c, x);
+      float(&f)[VEC] = HELD ? f2[HELD ? i : 0] : x;
       v_mul<VEC>(u[i], u[i], r2);
-      v_mul<VEC>(u[i], u[i], w);
+      v_mul<VEC>(u[i], u[i], f);
       store_pack<T, VEC>(static_cast<T*>(a.n) + out + c, u[i]);
     }
   }
@@ -191,17 +219,20 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) 
 }
 
 template <typename T, int VEC, int VPT, int MAXT>
-__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) norm_backward_kernel(const b200_norm_args a) {
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_backward_kernel(const b200_norm_args a) {
   extern __shared__ uint4 slots[];
-  __shared__ __align__(16) float sums[2][3][32];
+  __shared__ __align__(16) float sums[2][2][32];
   constexpr bool WARP_ROW = MAXT == 32;
   constexpr int S = NORM_STAGES<true, VEC, VPT, MAXT>;
+  constexpr int VQ = VEC / 4;                              // float4 of a pack's column factors
   const int part = WARP_ROW ? blockIdx.x * NORM_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
   const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
   const int threads = blockDim.x, stride = (WARP_ROW ? 32 : threads) * VEC;
   const float inv_h = 1.f / static_cast<float>(a.H);
   const bool next = a.dn != nullptr;
-  uint4* mine = slots + threadIdx.x;                       // [stage][y, dh, res, dn][VPT][threads]
+  // [w times gate, w2][VPT][VQ][threads], then [stage][y, dh, res, dn][VPT][threads]: a thread's own, all of them
+  float4* factors = reinterpret_cast<float4*>(slots) + threadIdx.x;
+  uint4* mine = slots + (S > 0 ? 2 * VPT * VQ * threads : 0) + threadIdx.x;
   const int tensors = next ? 4 : 2;
   auto at = [&](int stage, int tensor) { return mine + (stage * tensors + tensor) * VPT * threads; };
   auto fetch = [&](int row, int stage) {
@@ -217,12 +248,41 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) n
       async_commit();
     }
   };
-  if constexpr (!WARP_ROW) {
-    for (int i = threadIdx.x; i < 192; i += threads) (&sums[0][0][0])[i] = 0.f;
-    __syncthreads();
-  }
 #pragma unroll
   for (int s = 0; s < S; ++s) fetch(part + s * a.parts, s);
+  if constexpr (!WARP_ROW) {
+    for (int i = threadIdx.x; i < 128; i += threads) (&sums[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
+  auto factor = [&](int which, int i, int c, float (&f)[VEC]) {
+    if constexpr (S > 0) {
+#pragma unroll
+      for (int q = 0; q < VQ; ++q) {
+        const float4 x = factors[((which * VPT + i) * VQ + q) * threads];
+        f[4 * q] = x.x; f[4 * q + 1] = x.y; f[4 * q + 2] = x.z; f[4 * q + 3] = x.w;
+      }
+    } else if (which == 0) {
+      column_factor<T, VEC>(a, c, f);
+    } else {
+      load_param<T, VEC>(a.w2, a.w2_f32, c, f);
+    }
+  };
+  if constexpr (S > 0) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t * VEC + i * stride;
+      if (c >= a.H) continue;
+      float f[VEC];
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        if (which == 0) column_factor<T, VEC>(a, c, f);
+        else if (next) load_param<T, VEC>(a.w2, a.w2_f32, c, f);
+#pragma unroll
+        for (int q = 0; q < VQ; ++q)
+          factors[((which * VPT + i) * VQ + q) * threads] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+      }
+    }
+  }
 
   float acc[VPT][VEC], acc2[VPT][VEC];
 #pragma unroll
@@ -230,30 +290,26 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) n
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[i][j] = acc2[i][j] = 0.f;
 
+  // a row's three numbers, read while the row before is in work
+  float n1 = 1.f, n2 = 0.f, ng = 1.f;
+  auto numbers = [&](int row) {
+    if (row >= a.T) return;
+    if (a.norm) n1 = a.r1[row];
+    if (next) n2 = a.r2[row];
+    ng = row_factor<T>(a, row);
+  };
+  numbers(part);
+
   int set = 0, stage = 0;
   for (int row = part; row < a.T; row += a.parts, set ^= 1, stage = stage + 1 >= S ? 0 : stage + 1) {
     if constexpr (S > 0) async_wait<S - 1>();
-    const float r1 = a.norm ? a.r1[row] : 1.f;
-    const float r2 = next ? a.r2[row] : 0.f;
-    float gate_row[1] = {1.f};
-    if (a.gate_kind == 2) load_param<T, 1>(a.gate, a.gate_f32, static_cast<size_t>(row) * a.ld_gate, gate_row);
-    // x *= the gate's values of a pack
-    auto times_gate = [&](int c, float (&x)[VEC]) {
-      if (a.gate_kind == 0) return;
-      if (a.gate_kind == 2) {
-        v_mul<VEC>(x, x, gate_row[0]);
-        return;
-      }
+    const float r1 = n1, r2 = n2, gate_row = ng;
+    numbers(row + a.parts);
+    auto times_full_gate = [&](int c, float (&x)[VEC]) {
+      if (a.gate_kind != 3) return;
       float g[VEC];
-      if (a.gate_kind == 1) load_param<T, VEC>(a.gate, a.gate_f32, c, g);
-      else load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
+      load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
       v_mul<VEC>(x, x, g);
-    };
-    auto times_weight = [&](int c, float (&x)[VEC]) {
-      if (a.w == nullptr) return;
-      float w[VEC];
-      load_param<T, VEC>(a.w, a.w_f32, c, w);
-      v_mul<VEC>(x, x, w);
     };
     float yh[VPT][VEC], hh[VPT][VEC], gh[VPT][VEC];
     float m[2] = {0.f, 0.f};
@@ -264,30 +320,30 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) n
       for (int j = 0; j < VEC; ++j) yh[i][j] = hh[i][j] = gh[i][j] = 0.f;
       if (c >= a.H) continue;
       read_pack<T, VEC, S>(at(stage, 0) + i * threads, a.y, a.ld_y, row, c, yh[i]);
-      if (a.norm) v_mul<VEC>(yh[i], yh[i], r1);
+      v_mul<VEC>(yh[i], yh[i], r1);
       if (next) {
-        float x[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] = yh[i][j];
-        times_weight(c, x);
-        times_gate(c, x);
+        float x[VEC], f[VEC];
         read_pack<T, VEC, S>(at(stage, 2) + i * threads, a.res, a.ld_res, row, c, hh[i]);
-        v_fma<VEC>(hh[i], hh[i], a.scale, x);
+        v_mul<VEC>(hh[i], hh[i], a.scale);
+        v_mul<VEC>(x, yh[i], gate_row);
+        times_full_gate(c, x);
+        factor(0, i, c, f);
+        v_fma<VEC>(hh[i], x, f, hh[i]);
         v_mul<VEC>(hh[i], hh[i], r2);
         read_pack<T, VEC, S>(at(stage, 3) + i * threads, a.dn, a.ld_dn, row, c, gh[i]);
         v_fma<VEC>(acc2[i], gh[i], hh[i], acc2[i]);
-        load_param<T, VEC>(a.w2, a.w2_f32, c, x);
-        v_mul<VEC>(gh[i], gh[i], x);
+        factor(1, i, c, f);
+        v_mul<VEC>(gh[i], gh[i], f);
         v_dot<VEC>(m, gh[i], hh[i]);
       }
     }
     const float mean = next ? row_sum<WARP_ROW>(m[0] + m[1], sums[set][0]) * inv_h : 0.f;
-    float mq[2] = {0.f, 0.f}, mg[2] = {0.f, 0.f};
+    m[0] = m[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t * VEC + i * stride;
       if (c >= a.H) continue;
-      float d[VEC];
+      float d[VEC], f[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) d[j] = 0.f;
       if (a.dh != nullptr) read_pack<T, VEC, S>(at(stage, 1) + i * threads, a.dh, a.ld_dh, row, c, d);
@@ -295,46 +351,43 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) n
         v_fma<VEC>(gh[i], hh[i], -mean, gh[i]);
         v_fma<VEC>(d, gh[i], r2, d);
       }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) gh[i][j] = d[j];
-      if (a.gate_kind >= 2) {                     // a gate that changes from row to row: its own gradient, and A takes it in
+      factor(0, i, c, f);
+      // A takes in a gate that changes from row to row; gh becomes q but for the row's gate
+      float g[VEC];
+      v_mul<VEC>(g, d, gate_row);
+      if (a.gate_kind == 3) {
         float p[VEC];
-        v_mul<VEC>(p, d, yh[i]);
-        times_weight(c, p);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) mg[j & 1] += p[j];
-        if (a.gate_kind == 3 && a.dgate != nullptr) store_pack<T, VEC>(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * a.H + c, p);
-        times_gate(c, gh[i]);
-        v_fma<VEC>(acc[i], gh[i], yh[i], acc[i]);
+        v_mul<VEC>(p, d, f);
+        v_mul<VEC>(p, p, yh[i]);
+        if (a.dgate != nullptr) store_pack<T, VEC>(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * a.H + c, p);
+        times_full_gate(c, g);
+        v_mul<VEC>(gh[i], g, f);
       } else {
-        v_fma<VEC>(acc[i], gh[i], yh[i], acc[i]);
-        times_gate(c, gh[i]);
+        v_mul<VEC>(gh[i], d, f);
       }
-      times_weight(c, gh[i]);                     // q
-      v_dot<VEC>(mq, gh[i], yh[i]);
+      v_fma<VEC>(acc[i], g, yh[i], acc[i]);
+      v_dot<VEC>(m, gh[i], yh[i]);
       if (a.dres != nullptr) {
         v_mul<VEC>(d, d, a.scale);
         store_pack<T, VEC>(static_cast<T*>(a.dres) + static_cast<size_t>(row) * a.H + c, d);
       }
     }
     fetch(row + S * a.parts, stage);
-    if (a.gate_kind == 2 && a.dgate != nullptr) {
-      const float g = row_sum<WARP_ROW>(mg[0] + mg[1], sums[set][1]);
-      if (t == 0) {
-        if (a.gate_f32) static_cast<float*>(a.dgate)[row] = g;
-        else static_cast<T*>(a.dgate)[row] = from_f32<T>(g);
-      }
+    const bool row_gate = a.gate_kind == 2 && a.dgate != nullptr;
+    float sum = 0.f;                                 // gate per row: its gradient, and the mean of q yh but for the gate
+    if (a.norm || row_gate) sum = row_sum<WARP_ROW>(m[0] + m[1], sums[set][1]);
+    if (row_gate && t == 0) {
+      if (a.gate_f32) static_cast<float*>(a.dgate)[row] = sum;
+      else static_cast<T*>(a.dgate)[row] = from_f32<T>(sum);
     }
-    const float mean_q = a.norm ? row_sum<WARP_ROW>(mq[0] + mq[1], sums[set][2]) * inv_h : 0.f;
     if (a.dy != nullptr) {
+      const float mean_q = a.norm ? sum * inv_h : 0.f, r = r1 * gate_row;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = t * VEC + i * stride;
         if (c >= a.H) continue;
-        if (a.norm) {
-          v_fma<VEC>(gh[i], yh[i], -mean_q, gh[i]);
-          v_mul<VEC>(gh[i], gh[i], r1);
-        }
+        v_fma<VEC>(gh[i], yh[i], -mean_q, gh[i]);
+        v_mul<VEC>(gh[i], gh[i], r);
         store_pack<T, VEC>(static_cast<T*>(a.dy) + static_cast<size_t>(row) * a.H + c, gh[i]);
       }
     }
@@ -397,10 +450,10 @@ static int norm_row_threads(int H, int vec, int vpt) {
 
 // Rows (of warps, or of blocks) in work at once: the blocks that the registers of the variant and the slots leave room
 // for on every SM, and no more rows than there are.
-template <bool BACK, int MAXT>
+template <int MAXT>
 static int norm_parts(int T, int threads, size_t smem, int sms) {
   const int rows = MAXT == 32 ? NORM_WARP_ROWS : 1;
-  int per_sm = MAXT == 32 ? NORM_BLOCKS<BACK, 32> : MAXT * NORM_BLOCKS<BACK, MAXT> / threads;
+  int per_sm = MAXT == 32 ? NORM_BLOCKS<32> : MAXT * NORM_BLOCKS<MAXT> / threads;
   const int fit = static_cast<int>((224u * 1024u) / (smem + 2048));      // beside 1 KB of the system's and the sums
   if (fit < per_sm) per_sm = fit > 0 ? fit : 1;
   const int blocks = (T + rows - 1) / rows;
@@ -412,8 +465,9 @@ static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
   const int threads = norm_row_threads<MAXT>(a.H, VEC, VPT);
   const int block = MAXT == 32 ? NORM_WARP_ROWS * 32 : threads;
   const int tensors = BACK ? (a.dn != nullptr ? 4 : 2) : (a.res != nullptr ? 2 : 1);
-  const size_t smem = static_cast<size_t>(NORM_STAGES<BACK, VEC, VPT, MAXT>) * tensors * VPT * block * 16;      // at most 192 KB
-  a.parts = norm_parts<BACK, MAXT>(a.T, threads, smem, sms);
+  constexpr int S = NORM_STAGES<BACK, VEC, VPT, MAXT>;
+  const size_t smem = (static_cast<size_t>(S) * tensors * VPT * 16 + (BACK && S > 0 ? 2 * VPT * VEC * 4 : 0)) * block;   // at most 200 KB
+  a.parts = norm_parts<MAXT>(a.T, threads, smem, sms);
   const dim3 grid(MAXT == 32 ? a.parts / NORM_WARP_ROWS : a.parts);
   auto kern = BACK ? norm_backward_kernel<T, VEC, VPT, MAXT> : norm_forward_kernel<T, VEC, VPT, MAXT>;
   if (smem > 40 * 1024) {          // 48 KB, static shared memory included, need no leave
@@ -462,7 +516,7 @@ static int norm_dispatch(bool back, const b200_norm_args& a, int sms, cudaStream
 struct NormPartsOf {
   int T, H, sms;
   template <int VEC, int VPT, int MAXT>
-  int operator()() const { return norm_parts<true, MAXT>(T, norm_row_threads<MAXT>(H, VEC, VPT), 0, sms); }
+  int operator()() const { return norm_parts<MAXT>(T, norm_row_threads<MAXT>(H, VEC, VPT), 0, sms); }
 };
 
 template <bool BACK>
