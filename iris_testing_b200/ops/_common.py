@@ -43,13 +43,10 @@ def contiguous_bf16(t: torch.Tensor, name: str) -> torch.Tensor:
 ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def require_elem(t: torch.Tensor, name: str, allowed=tuple(ELEM)) -> None:
-    require(t.dtype in allowed, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in allowed)} (got {t.dtype})")
-
-
 def require_device(device: torch.device, **tensors) -> None:
     for name, t in tensors.items():
-        require(t is None or t.device == device, f"{name} must be on {device} (got {t.device if t is not None else None})")
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device} (got {t.device})")
 
 
 class _Here:
@@ -70,8 +67,24 @@ def on_device(t: torch.Tensor):
 
 def rows_view(t: torch.Tensor) -> torch.Tensor:
     """``t`` as [rows, last dim] with unit stride along a row; a copy only where no such view exists."""
-    v = t.reshape(-1, t.shape[-1])
-    return v if v.shape[-1] == 1 or v.stride(-1) == 1 else v.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+class Entry:
+    """One exported function, looked up and declared at its first call; a non-zero code raises."""
+
+    def __init__(self, name: str, *argtypes):
+        self.name, self.argtypes, self.fn = name, argtypes, None
+
+    def __call__(self, *args) -> None:
+        fn = self.fn
+        if fn is None:
+            fn = self.fn = declare(self.name, list(self.argtypes))
+        code = fn(*args)
+        if code != 0:
+            nv.check(code, self.name.replace("b200_", "").replace("_", " ") + " launch")
 
 
 _declared = set()

@@ -11,8 +11,8 @@ import torch
 
 from .. import _native as nv
 from . import cpu_ref
-from ._common import (ELEM, declare, launch_status, on_device, ptr, require, require_device, require_elem, rows_view,
-                      stream_ptr, use_native)
+from ._common import (ELEM, Entry, declare, launch_status, on_device, require, require_device, rows_view, stream_ptr,
+                      use_native)
 from .expert import sm_count
 
 MAX_BALANCE_EXPERTS = 1024
@@ -25,54 +25,56 @@ class BalanceArgs(C.Structure):
         + [("coef", C.c_float), ("z", C.c_float)]
 
 
+_FORWARD = Entry("b200_balance_forward", C.POINTER(BalanceArgs), C.c_void_p)
+_BACKWARD = Entry("b200_balance_backward", C.POINTER(BalanceArgs), C.c_void_p)
+_I32, _F32 = torch.int32, torch.float32
+
+
 def _fill(logits, k, seq_rows, mask, coef, z, S):
     a = BalanceArgs()
-    a.T, a.E = logits.shape
-    a.k, a.S, a.elem, a.coef, a.z = k, S, ELEM[logits.dtype], coef, z
+    T, E = logits.shape
+    elem = ELEM[logits.dtype]
+    a.T, a.E, a.k, a.S, a.elem, a.coef, a.z = T, E, k, S, elem, coef, z
     a.logits, a.ld = logits.data_ptr(), logits.stride(0)
-    a.seq_rows = None if seq_rows is None else seq_rows.data_ptr()
-    a.mask = None if mask is None else mask.data_ptr()
-    runs = declare("b200_balance_runs", [C.c_int] * 4)(a.T, a.E, a.elem, sm_count(logits.device))
-    a.run_tokens = -(-a.T // runs)
-    a.runs = -(-a.T // a.run_tokens)
     if seq_rows is not None:
-        a.status = launch_status(logits.device).data_ptr()
+        a.seq_rows, a.status = seq_rows.data_ptr(), launch_status(logits.device).data_ptr()
+    if mask is not None:
+        a.mask = mask.data_ptr()
+    runs = declare("b200_balance_runs", [C.c_int] * 4)(T, E, elem, sm_count(logits.device))
+    a.run_tokens = tokens = -(-T // runs)
+    a.runs = -(-T // tokens)
     return a
 
 
-def _call(name, a, t):
-    fn = declare(name, [C.POINTER(BalanceArgs), C.c_void_p])
-    with on_device(t):
-        nv.check(fn(C.byref(a), stream_ptr(t)), name.replace("b200_", "").replace("_", " ") + " launch")
-
-
 def _forward(logits, idx, seq_rows, mask, coef, z):
-    """(loss, counts [S, E], what the backward pass reads)."""
+    """(loss, counts [E] or [S, E], scratch that holds what the backward pass reads, or None)."""
     T, E = logits.shape
-    S = 1 if seq_rows is None else seq_rows.numel()
     dev = logits.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    counts = torch.empty((S, E), dtype=torch.int32, device=dev)
+    S = 1 if seq_rows is None else seq_rows.numel()
+    loss = torch.empty((), dtype=_F32, device=dev)
+    counts = torch.empty((E,) if seq_rows is None else (S, E), dtype=_I32, device=dev)
     if T == 0 or S == 0:
         return loss.zero_(), counts.zero_(), None
     a = _fill(logits, idx.shape[1], seq_rows, mask, coef, z, S)
-    keep = torch.empty(S * E + S + 2, dtype=torch.int32, device=dev)          # counts, tokens per sequence, two fp32 words
-    parts = S * -(-E // 32)
-    work = torch.empty((a.runs + S) * (2 * E + 2) + parts + S + 1, dtype=torch.float32, device=dev)
+    # kept counts, tokens per sequence, two fp32 words; then the records, parts of the terms, z sums and a ticket
+    parts, kept, records = S * -(-E // 32), S * E + S + 2, (a.runs + S) * (2 * E + 2)
+    work = torch.empty(kept + records + parts + S + 1, dtype=_I32, device=dev)
     a.idx, a.loss, a.counts = idx.data_ptr(), loss.data_ptr(), counts.data_ptr()
-    a.record = work.data_ptr()
-    a.seq_loss = a.record + 4 * (a.runs + S) * (2 * E + 2)
-    a.seq_z = a.seq_loss + 4 * parts
-    a.ticket = a.seq_z + 4 * S
-    _keep(a, keep, S, E)
-    _call("b200_balance_forward", a, logits)
-    return loss, counts, keep
+    base = work.data_ptr()
+    _keep(a, base, S, E)
+    a.record = p = base + 4 * kept
+    a.seq_loss = p = p + 4 * records
+    a.seq_z = p = p + 4 * parts
+    a.ticket = p + 4 * S
+    with on_device(logits):
+        _FORWARD(a, stream_ptr(logits))
+    return loss, counts, work
 
 
-def _keep(a, keep, S, E):
-    a.kept = keep.data_ptr()
-    a.seq_tokens = a.kept + 4 * S * E
-    a.total = a.seq_tokens + 4 * S
+def _keep(a, base, S, E):
+    a.kept = base
+    a.seq_tokens = base + 4 * S * E
+    a.total = base + 4 * S * (E + 1)
 
 
 class _Balance(torch.autograd.Function):
@@ -97,10 +99,12 @@ class _Balance(torch.autograd.Function):
         k, coef, z = ctx.how
         S = 1 if seq_rows is None else seq_rows.numel()
         a = _fill(logits, k, seq_rows, mask, coef, z, S)
-        _keep(a, keep, S, logits.shape[1])
-        dloss = dloss.float().contiguous()
+        _keep(a, keep.data_ptr(), S, logits.shape[1])
+        if dloss.dtype != _F32:
+            dloss = dloss.float()
         a.grad_loss, a.grad = dloss.data_ptr(), grad.data_ptr()
-        _call("b200_balance_backward", a, logits)
+        with on_device(logits):
+            _BACKWARD(a, stream_ptr(logits))
         return (grad,) + (None,) * 5
 
 
@@ -132,16 +136,17 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
     if not use_native(logits):
         loss, counts = cpu_ref.balance_loss_ref(logits, topk_idx, balance_coef, z_coef, seq_rows, token_mask)
         return loss, counts if seq_rows is not None else counts[0]
-    require_elem(logits, "logits")
-    require(E <= MAX_BALANCE_EXPERTS, f"at most {MAX_BALANCE_EXPERTS} experts (got {E})")
+    if logits.dtype not in ELEM:
+        raise ValueError(f"logits must be float32, bfloat16 or float16 (got {logits.dtype})")
+    if E > MAX_BALANCE_EXPERTS:
+        raise ValueError(f"at most {MAX_BALANCE_EXPERTS} experts (got {E})")
     require_device(logits.device, topk_idx=topk_idx, seq_rows=seq_rows, token_mask=token_mask)
-    logits = rows_view(logits)
-    idx = topk_idx.contiguous()
-    rows = None if seq_rows is None else seq_rows.contiguous()
-    mask = None if token_mask is None else token_mask.contiguous()
+    logits, idx = rows_view(logits), topk_idx.contiguous()
+    if seq_rows is not None:
+        seq_rows = seq_rows.contiguous()
+    if token_mask is not None:
+        token_mask = token_mask.contiguous()
     how = (float(balance_coef), float(z_coef))
     if torch.is_grad_enabled() and logits.requires_grad:
-        loss, counts = _Balance.apply(logits, idx, rows, mask, *how)
-    else:
-        loss, counts, _ = _forward(logits, idx, rows, mask, *how)
-    return loss, counts if seq_rows is not None else counts[0]
+        return _Balance.apply(logits, idx, seq_rows, token_mask, *how)
+    return _forward(logits, idx, seq_rows, token_mask, *how)[:2]

@@ -13,7 +13,7 @@ import torch
 
 from .. import _native as nv
 from . import cpu_ref
-from ._common import ELEM, declare, launch_status, on_device, require, require_device, require_elem, stream_ptr, use_native
+from ._common import ELEM, Entry, launch_status, on_device, require, require_device, stream_ptr, use_native
 from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
@@ -30,6 +30,10 @@ class LinearArgs(C.Structure):
 class ActGradArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "dz", "dres", "dbias", "record", "group_rows")] \
         + [(n, C.c_int) for n in ("G", "M", "N", "n_out", "elem", "act", "chunks", "chunk_rows")]
+
+
+_PRODUCT = Entry("b200_linear", C.POINTER(LinearArgs), C.c_int, C.c_void_p)
+_ACT_GRAD = Entry("b200_act_grad", C.POINTER(ActGradArgs), C.c_void_p)
 
 
 def _plain(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -49,16 +53,19 @@ def _pairs(mode: int, M: int, N: int, K: int, G: int) -> bool:
 def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, res=None):
     la = LinearArgs()
     la.a, la.b, la.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
-    la.z = None if z is None else z.data_ptr()
-    la.bias = None if bias is None else bias.data_ptr()
-    la.res = None if res is None else res.data_ptr()
-    la.group_rows = None if group_rows is None else group_rows.data_ptr()
+    if z is not None:
+        la.z = z.data_ptr()
+    if bias is not None:
+        la.bias = bias.data_ptr()
+    if res is not None:
+        la.res = res.data_ptr()
+    if group_rows is not None:
+        la.group_rows = group_rows.data_ptr()
     la.status = launch_status(a.device).data_ptr()
     la.wait_budget_ns = 2_000_000_000
     la.mode, la.G, la.M, la.N, la.K, la.n_out = mode, G, M, N, K, out.shape[-1]
     la.elem, la.act, la.pair = ELEM[a.dtype], act, int(_pairs(mode, M, N, K, G))
-    fn = declare("b200_linear", [C.POINTER(LinearArgs), C.c_int, C.c_void_p])
-    nv.check(fn(C.byref(la), sm_count(a.device), stream_ptr(a)), "linear launch")
+    _PRODUCT(la, sm_count(a.device), stream_ptr(a))
 
 
 def _forward(x, w, bias, residual, group_rows, act, save):
@@ -102,8 +109,7 @@ def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
             if db is not None:
                 record = torch.empty((a.chunks + G, N), dtype=torch.float32, device=dev)
                 a.dbias, a.record = db.data_ptr(), record.data_ptr()
-            fn = declare("b200_act_grad", [C.POINTER(ActGradArgs), C.c_void_p])
-            nv.check(fn(C.byref(a), stream_ptr(x)), "activation gradient launch")
+            _ACT_GRAD(a, stream_ptr(x))
         if dx is not None:
             _product(_DX, dz, w, dx, M, N, K, G, group_rows)
         if dw is not None:
@@ -144,7 +150,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     pre-activation and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
     timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.  CPU tensors take
     plain PyTorch."""
-    require(activation in ACTIVATIONS, f"activation must be one of {list(ACTIVATIONS)} (got {activation!r})")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)} (got {activation!r})")
     grouped = group_rows is not None
     require(w_kmajor.dim() == (3 if grouped else 2), "w_kmajor must be [N, K], or [G, N, K] with group_rows")
     N, K = w_kmajor.shape[-2:]
@@ -159,15 +166,17 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     require(residual is None or residual.shape == x.shape[:-1] + (n_out,), "residual must have the result's shape")
     require(not grouped or (group_rows.dtype == torch.int32 and group_rows.shape == (G,)),
             "group_rows must be int32 with one entry per group")
-    require(not grouped or 1 <= G <= nv.MAX_GROUPS, f"at most {nv.MAX_GROUPS} groups")
+    require(not grouped or 1 <= G <= nv.MAX_GROUPS, "too many groups (128 at most), or none")
     shape = x.shape[:-1] + (n_out,)
     if not use_native(x):
         require(not grouped or int(group_rows.clamp(min=0).sum()) <= x.shape[0], "the groups hold more rows than x")
         r = None if residual is None else residual.reshape(-1, n_out)
         return cpu_ref.linear_ref(x.reshape(-1, K), w_kmajor, bias, r, activation, group_rows).to(x.dtype).view(shape)
-    require_elem(x, "x", (torch.bfloat16, torch.float16))
-    for name, t in (("w_kmajor", w_kmajor), ("bias", bias), ("residual", residual)):
-        require(t is None or t.dtype == x.dtype, f"{name} must have x's dtype")
+    dt = x.dtype
+    if dt != torch.bfloat16 and dt != torch.float16:
+        raise ValueError(f"x must be bfloat16 or float16 (got {dt})")
+    require(w_kmajor.dtype == dt and (bias is None or bias.dtype == dt) and (residual is None or residual.dtype == dt),
+            "w_kmajor, bias and residual must have x's dtype")
     require(K % 8 == 0 and N % 8 == 0, "K and N must be multiples of 8")
     require(x.numel() // K < 2 ** 31 and G * N < 2 ** 31, "too many rows")
     require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)

@@ -12,8 +12,7 @@ import torch
 
 from .. import _native as nv
 from . import cpu_ref
-from ._common import (ELEM, declare, on_device, ptr, require, require_device, require_elem, rows_view, stream_ptr,
-                      use_native)
+from ._common import ELEM, Entry, declare, on_device, require, require_device, rows_view, stream_ptr, use_native
 from .expert import sm_count
 
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
@@ -28,102 +27,108 @@ class NormArgs(C.Structure):
         + [("scale", C.c_float), ("eps", C.c_float)]
 
 
-def _gate_kind(gate: Optional[torch.Tensor], shape) -> int:
-    if gate is None:
-        return GATE_NONE
+_FORWARD = Entry("b200_norm_forward", C.POINTER(NormArgs), C.c_int, C.c_void_p)
+_BACKWARD = Entry("b200_norm_backward", C.POINTER(NormArgs), C.c_int, C.c_void_p)
+_F32 = torch.float32
+
+
+def _gate_kind(gate: torch.Tensor, shape) -> int:
     if gate.shape == shape[-1:]:
         return GATE_CHANNEL
     if gate.shape == shape and shape[-1] > 1:     # of a single column, a gate per element is one per row
         return GATE_FULL
-    require(gate.shape == shape[:-1] + (1,),
-            f"gate must be one value per column {tuple(shape[-1:])}, per row {tuple(shape[:-1] + (1,))} or per element "
-            f"{tuple(shape)} (got {tuple(gate.shape)})")
+    if gate.shape != shape[:-1] + (1,):
+        raise ValueError(f"gate must be one value per column {tuple(shape[-1:])}, per row {tuple(shape[:-1] + (1,))} or per "
+                         f"element {tuple(shape)} (got {tuple(gate.shape)})")
     return GATE_ROW
 
 
-def _check(y, residual, weight, gate, next_weight):
-    require(y.dim() >= 1 and y.shape[-1] >= 1, "y must have at least one dimension, and columns in the last one")
-    H = y.shape[-1]
-    require(residual is None or residual.shape == y.shape, "residual must have y's shape")
-    for name, w in (("weight", weight), ("next_weight", next_weight)):
-        require(w is None or w.shape == (H,), f"{name} must have one value per column ({H})")
-    kind = _gate_kind(gate, y.shape)
-    if not use_native(y):
+def _check(y, residual, weight, gate, next_weight) -> int:
+    """Refuses what does not fit together; the kind of gate."""
+    shape = y.shape
+    require(len(shape) >= 1 and shape[-1] >= 1, "y must have at least one dimension, and columns in the last one")
+    H, dt = shape[-1], y.dtype
+    require(residual is None or residual.shape == shape, "residual must have y's shape")
+    require(weight is None or weight.shape == shape[-1:], "weight must have one value per column")
+    require(next_weight is None or next_weight.shape == shape[-1:], "next_weight must have one value per column")
+    kind = GATE_NONE if gate is None else _gate_kind(gate, shape)
+    if not y.is_cuda:
         return kind
-    require(H <= MAX_COLUMNS, f"at most {MAX_COLUMNS} columns (got {H})")
-    require(y.numel() // H <= 2 ** 30, "too many rows")
-    require_elem(y, "y")
-    require(residual is None or residual.dtype == y.dtype, "residual must have y's dtype")
-    for name, w in (("weight", weight), ("next_weight", next_weight), ("gate", gate if kind != GATE_FULL else None)):
-        require(w is None or w.dtype in (y.dtype, torch.float32), f"{name} must have y's dtype or be float32")
-    require(kind != GATE_FULL or gate.dtype == y.dtype, "a gate per element must have y's dtype")
+    if H > MAX_COLUMNS or y.numel() > H << 30:
+        raise ValueError(f"at most {MAX_COLUMNS} columns (got {H}) and 2^30 rows")
+    if dt not in ELEM:
+        raise ValueError(f"y must be float32, bfloat16 or float16 (got {dt})")
+    require(residual is None or residual.dtype == dt, "residual must have y's dtype")
+    require(weight is None or weight.dtype == dt or weight.dtype == _F32, "weight must have y's dtype or be float32")
+    require(next_weight is None or next_weight.dtype == dt or next_weight.dtype == _F32,
+            "next_weight must have y's dtype or be float32")
+    require(kind == GATE_NONE or gate.dtype == dt or (gate.dtype == _F32 and kind != GATE_FULL),
+            "gate must have y's dtype, or be float32 where it is one value per column or row")
     require_device(y.device, residual=residual, weight=weight, gate=gate, next_weight=next_weight)
     return kind
 
 
 def _fill(y, residual, weight, gate, kind, norm, scale, next_weight, eps, keep):
-    """Argument block of one call and the number of rows; ``keep`` holds what has to outlive the launch."""
+    """Argument block of one call; ``keep`` holds what has to outlive the launch."""
     a = NormArgs()
-    a.H, a.elem, a.norm, a.gate_kind, a.scale, a.eps = y.shape[-1], ELEM[y.dtype], int(norm), kind, scale, eps
-
-    def rows(t):
-        v = rows_view(t)
-        keep.append(v)
-        return v, v.data_ptr(), (v.stride(0) if v.shape[0] > 1 else v.shape[1])
-
-    def vector(t):
-        v = t if t.is_contiguous() else t.contiguous()
-        keep.append(v)
-        return v.data_ptr(), int(t.dtype == torch.float32)
-
-    y2, a.y, a.ld_y = rows(y)
-    a.T = y2.shape[0]
+    H, size = y.shape[-1], y.element_size()
+    a.H, a.elem, a.norm, a.gate_kind, a.scale, a.eps = H, ELEM[y.dtype], norm, kind, scale, eps
+    y = rows_view(y)
+    T = a.T = y.shape[0]
+    ld = H if T == 1 else y.stride(0)
+    p = y.data_ptr()
+    a.y, a.ld_y, bits, lds = p, ld, p, H | ld
+    keep.append(y)
     if residual is not None:
-        _, a.res, a.ld_res = rows(residual)
+        residual = rows_view(residual)
+        ld = H if T == 1 else residual.stride(0)
+        p = residual.data_ptr()
+        a.res, a.ld_res, bits, lds = p, ld, bits | p, lds | ld
+        keep.append(residual)
     if weight is not None:
-        a.w, a.w_f32 = vector(weight)
+        weight = weight.contiguous()
+        a.w = p = weight.data_ptr()
+        a.w_f32, bits = weight.dtype == _F32, bits | p
+        keep.append(weight)
     if next_weight is not None:
-        a.w2, a.w2_f32 = vector(next_weight)
-    if kind == GATE_CHANNEL:
-        a.gate, a.gate_f32 = vector(gate)
-    elif kind != GATE_NONE:
-        _, a.gate, a.ld_gate = rows(gate)
-        a.gate_f32 = int(gate.dtype == torch.float32)
+        next_weight = next_weight.contiguous()
+        a.w2 = p = next_weight.data_ptr()
+        a.w2_f32, bits = next_weight.dtype == _F32, bits | p
+        keep.append(next_weight)
+    if kind != GATE_NONE:
+        a.gate_f32 = gate.dtype == _F32
+        if kind == GATE_CHANNEL:
+            gate = gate.contiguous()
+            bits |= gate.data_ptr()
+        else:
+            gate = rows_view(gate)
+            a.ld_gate = ld = gate.shape[1] if T == 1 else gate.stride(0)
+            if kind == GATE_FULL:
+                bits, lds = bits | gate.data_ptr(), lds | ld
+        a.gate = gate.data_ptr()
+        keep.append(gate)
+    # whole 16-byte packs are moved where every row of every tensor starts on one
+    a.aligned = bits % 16 == 0 and lds * size % 16 == 0
     return a
-
-
-def _align(a: NormArgs, size: int) -> None:
-    """Whole 16-byte packs are moved where every row of every tensor starts on one."""
-    bits = (a.y or 0) | (a.res or 0) | (a.w or 0) | (a.w2 or 0) | (a.dh or 0) | (a.dn or 0)
-    lds = a.H | a.ld_y | a.ld_res | a.ld_dh | a.ld_dn
-    if a.gate_kind in (GATE_CHANNEL, GATE_FULL):
-        bits |= a.gate
-    if a.gate_kind == GATE_FULL:
-        lds |= a.ld_gate
-    a.aligned = int(bits % 16 == 0 and lds * size % 16 == 0)
-
-
-def _call(name, a, t):
-    fn = declare(name, [C.POINTER(NormArgs), C.c_int, C.c_void_p])
-    with on_device(t):
-        nv.check(fn(C.byref(a), sm_count(t.device), stream_ptr(t)), name.replace("b200_", "").replace("_", " ") + " launch")
 
 
 def _forward(y, residual, weight, gate, kind, norm, scale, next_weight, eps, save):
     h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     n = None if next_weight is None else torch.empty_like(h)
     T = y.numel() // y.shape[-1]
-    stats = torch.empty((2, T), dtype=torch.float32, device=y.device) if save else None
+    stats = torch.empty((2, T), dtype=_F32, device=y.device) if save else None
     if T == 0:
         return h, n, stats
     keep = []
     a = _fill(y, residual, weight, gate, kind, norm, scale, next_weight, eps, keep)
-    a.h, a.n = h.data_ptr(), None if n is None else n.data_ptr()
+    a.h = h.data_ptr()
+    if n is not None:
+        a.n = n.data_ptr()
     if save:
-        a.r1 = stats.data_ptr()
-        a.r2 = a.r1 + 4 * T
-    _align(a, y.element_size())
-    _call("b200_norm_forward", a, y)
+        a.r1 = p = stats.data_ptr()
+        a.r2 = p + 4 * T
+    with on_device(y):
+        _FORWARD(a, sm_count(y.device), stream_ptr(y))
     return h, n, stats
 
 
@@ -131,30 +136,35 @@ def _backward(saved, kind, norm, scale, eps, need, dh, dn):
     """Gradients of (y, residual, weight, gate, next_weight), None where ``need`` says so."""
     y, residual, weight, gate, next_weight, stats = saved
     like = (y, residual, weight, gate, next_weight)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and n else None for t, n in zip(like, need)]
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n and t is not None else None for t, n in zip(like, need)]
     T = y.numel() // y.shape[-1]
     if T == 0 or (dh is None and dn is None):
         return [None if g is None else g.zero_() for g in grads]
     keep = []
     a = _fill(y, residual, weight, gate, kind, norm, scale, next_weight, eps, keep)
-    for name, t in (("dh", dh), ("dn", dn)):
-        if t is not None:
-            v = rows_view(t)
-            keep.append(v)
-            setattr(a, name, v.data_ptr())
-            setattr(a, "ld_" + name, v.stride(0) if T > 1 else v.shape[1])
-    if dn is None and grads[4] is not None:       # the second output has no gradient
+    bits = lds = 0
+    if dh is not None:
+        dh = rows_view(dh)
+        a.dh, a.ld_dh = bits, lds = dh.data_ptr(), dh.stride(0) if T > 1 else dh.shape[1]
+    if dn is not None:
+        dn = rows_view(dn)
+        p, ld = dn.data_ptr(), dn.stride(0) if T > 1 else dn.shape[1]
+        a.dn, a.ld_dn, bits, lds = p, ld, bits | p, lds | ld
+    elif grads[4] is not None:                    # the second output has no gradient
         grads[4].zero_()
+    a.aligned = a.aligned and bits % 16 == 0 and lds * y.element_size() % 16 == 0
     a.dy, a.dres, a.dw, a.dgate = (None if g is None else g.data_ptr() for g in grads[:4])
-    a.dw2 = None if grads[4] is None or dn is None else grads[4].data_ptr()
-    a.r1 = stats.data_ptr()
-    a.r2 = a.r1 + 4 * T
-    _align(a, y.element_size())
+    if grads[4] is not None and dn is not None:
+        a.dw2 = grads[4].data_ptr()
+    a.r1 = p = stats.data_ptr()
+    a.r2 = p + 4 * T
+    sms = sm_count(y.device)
     if a.dw or a.dw2 or (a.dgate and kind == GATE_CHANNEL):
-        parts = declare("b200_norm_parts", [C.c_int] * 5)(T, a.H, a.elem, a.aligned, sm_count(y.device))
-        partial = torch.empty((2, parts, a.H), dtype=torch.float32, device=y.device)
+        parts = declare("b200_norm_parts", [C.c_int] * 5)(T, a.H, a.elem, a.aligned, sms)
+        partial = torch.empty((2, parts, a.H), dtype=_F32, device=y.device)
         a.partial = partial.data_ptr()
-    _call("b200_norm_backward", a, y)
+    with on_device(y):
+        _BACKWARD(a, sms, stream_ptr(y))
     return grads
 
 
