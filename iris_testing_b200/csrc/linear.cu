@@ -10,9 +10,9 @@
 // (x and W forward, dz for dX); the others (W for dX, both of dW) are read as they lie in memory, MN-major, in boxes of 64
 // columns x 64 contracted rows, so that nothing is ever transposed in memory.
 //
-// dW contracts over a group's rows, whose end lies anywhere inside a block of 64.  The rows of the last block that
-// belong to the next group (or to nothing) are set to zero in shared memory, in both operands, so that what lies there,
-// infinities and NaN included, has no part in the product.
+// dW contracts over a group's rows, whose end lies anywhere inside a block of 64.  The last block is multiplied as far as it
+// has rows, in steps of 16; the rows of the last step that belong to the next group (or to nothing) are set to zero in
+// shared memory, in both operands, so that what lies there, infinities and NaN included, has no part in the product.
 //
 // The hidden pre-activations z are kept for the backward pass in the element type; dz is rounded to it too, since the
 // tensor cores multiply 16-bit values: two roundings of half a step each that average out over the contracted dimension.
@@ -77,14 +77,15 @@ constexpr int LIN_A_BYTES = LBM * LBK * 2;
 constexpr int LIN_MN_BOX = 64 * LBK * 2; // bytes of one MN-major box
 constexpr int LIN_BOX = 32 * 128;        // a warp's staging box: 32 rows x 64 columns, 16-byte chunks XOR-swizzled by row
 
-// Stages and staging boxes per variant.  Forward: three boxes per epilogue warp (z of the gate, z of the up half, y);
-// the products without z need one.
+// Stages and staging boxes per variant.  An epilogue warp's boxes form a ring, so that it fills one while bulk stores still
+// read others (with one box, a 256 x 256 tile took 3.2 us to drain).  Forward, a pass fills up to three (z of the
+// gate, z of the up half, y).
 template <int MODE, int CG>
 struct LinGeo {
   static constexpr int B_ROWS = LBN / CG;
   static constexpr int B_BYTES = B_ROWS * LBK * 2;
   static constexpr int STAGE = LIN_A_BYTES + B_BYTES;
-  static constexpr int BOXES = MODE == LIN_FORWARD ? 3 : 1;
+  static constexpr int BOXES = MODE == LIN_FORWARD ? 4 : 2;
   static constexpr int STAGES = CG == 2 ? (MODE == LIN_FORWARD ? 5 : 6) : (MODE == LIN_FORWARD ? 3 : 4);
   static constexpr int TM = LBM * CG;
 };
@@ -179,28 +180,24 @@ __device__ __forceinline__ long long lin_scan(LinControl& c, const int* group_ro
 }
 
 // Writes one staging box: 32 rows x 64 columns at (row, col) of a row-major matrix.  Whole boxes leave as one bulk tensor
-// store, others row segment by row segment.
-__device__ __forceinline__ void store_box(uint8_t* box, const CUtensorMap* tmap, char* base, long long ld_bytes, long long row,
-                                          int col, int cols, int rows_here, int lane, bool& pending) {
+// store, others row segment by row segment; either way the box is one bulk group of lane 0.
+__device__ __forceinline__ void store_box(const uint8_t* box, const CUtensorMap* tmap, char* base, long long ld_bytes, long long row,
+                                          int col, int cols, int rows_here, int lane) {
   if (rows_here >= 32) {
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0 && col < cols) {
-      tma_store_2d(tmap, box, col, static_cast<int>(row));
-      bulk_commit_group();
-      pending = true;
-    }
-    return;
-  }
-  __syncwarp();
-  const int c = col + (lane & 7) * 8;
+    if (lane == 0 && col < cols) tma_store_2d(tmap, box, col, static_cast<int>(row));
+  } else {
+    __syncwarp();
+    const int c = col + (lane & 7) * 8;
 #pragma unroll
-  for (int rr = 0; rr < 8; ++rr) {
-    const int r = rr * 4 + (lane >> 3);
-    if (r < rows_here && c < cols)
-      st_16(base + (row + r) * ld_bytes + c * 2ll, *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4)));
+    for (int rr = 0; rr < 8; ++rr) {
+      const int r = rr * 4 + (lane >> 3);
+      if (r < rows_here && c < cols)
+        st_16(base + (row + r) * ld_bytes + c * 2ll, *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4)));
+    }
   }
-  __syncwarp();
+  if (lane == 0) bulk_commit_group();
 }
 
 template <int MODE, int CG, bool GATED>
@@ -280,7 +277,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 
   // blocks of the contracted dimension in a tile of group g
   auto k_blocks = [&](int g) { return ((MODE == LIN_FORWARD ? la.K : MODE == LIN_DX ? la.N : c.g_rows[g]) + LBK - 1) / LBK; };
-  // dW: contracted rows in the last block of group g (64: whole)
+  // dW: contracted rows in the last block of group g (64: whole); a number that is no multiple of 16 has to be mended
   auto tail_rows = [&](int g) { return MODE == LIN_DW ? ((c.g_rows[g] - 1) & (LBK - 1)) + 1 : LBK; };
 
   if (warp == 0) {
@@ -293,7 +290,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         int g, m, n;
         if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
         const int KB = k_blocks(g);
-        const bool ragged = tail_rows(g) < LBK;
+        const bool ragged = tail_rows(g) % 16 != 0;
         const int mrow = m * S::TM + static_cast<int>(cta_rank) * LBM;      // first row (dW: feature) of my half
         const int ncol = n * LBN + static_cast<int>(cta_rank) * S::B_ROWS;  // first column of my share of B
         const int row0 = c.g_row_start[g];
@@ -380,14 +377,15 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         int g, m, n;
         if (!decode_tile(c, G, TN, la.group_m, idx, cursor, g, m, n)) break;
         const int KB = k_blocks(g);
-        const bool ragged = tail_rows(g) < LBK;
+        const int tail = tail_rows(g);
         const int acc = it & 1;
         if (!mbar_wait(&c.tmem_empty[acc], ((it >> 1) & 1) ^ 1u, w, ST_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after_sync();
         const uint32_t d = tmem_base + acc * LBN;
         for (int kb = 0; kb < KB; ++kb) {
           if (!mbar_wait(&c.full[stage], phase, w, ST_TIMEOUT_PIPE_FULL)) { ok = false; break; }
-          if (MODE == LIN_DW && ragged && kb == KB - 1) {
+          const bool end = MODE == LIN_DW && kb == KB - 1;
+          if (end && tail % 16 != 0) {
             if (!mbar_wait_cluster(&c.mended[stage], mend_phase >> stage & 1u, w, ST_TIMEOUT_PIPE_FULL)) { ok = false; break; }
             mend_phase ^= 1u << stage;
           }
@@ -399,6 +397,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
           constexpr int ASTEP = A_MN ? 2048 / 16 : 2, BSTEP = B_MN ? 2048 / 16 : 2;
 #pragma unroll
           for (int k = 0; k < LBK / 16; ++k) {
+            if (end && k * 16 >= tail) continue;
             if constexpr (CG == 2) umma_bf16_ss_pair(d, ad + ASTEP * k, bd + BSTEP * k, idesc, (kb | k) != 0 ? 1u : 0u);
             else umma_bf16_ss(d, ad + ASTEP * k, bd + BSTEP * k, idesc, (kb | k) != 0 ? 1u : 0u);
           }
@@ -422,9 +421,13 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     constexpr int OUT_TILE = GATED ? LBN / 2 : LBN;
     const int q = warp & 3;                            // TMEM lane quarter this warp may read
     uint8_t* boxes = staging + q * S::BOXES * LIN_BOX;
-    uint8_t* ybox = boxes;
-    uint8_t* zbox = boxes + LIN_BOX;                   // forward: z, or the gate's z with the up half's behind it
-    bool pending = false;                              // lane 0: a bulk store may still be reading a box
+    int ring = 0;                                      // the next box
+    const bool save_z = MODE == LIN_FORWARD && la.z != nullptr;
+    auto take_box = [&]() {
+      uint8_t* box = boxes + ring * LIN_BOX;
+      ring = ring + 1 == S::BOXES ? 0 : ring + 1;
+      return box;
+    };
     int cursor = 0, it = 0;
     const uint32_t empty_addr[2] = {map_to_cta(&c.tmem_empty[0], 0), map_to_cta(&c.tmem_empty[1], 0)};
     for (int idx = tile_first; idx < total_tiles; idx += tile_stride, ++it) {
@@ -443,9 +446,16 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 #pragma unroll 1
       for (int p = 0; p < OUT_TILE / 64; ++p) {
         const int ycol = n * OUT_TILE + p * 64;        // first output column of the pass
-        if (pending) bulk_wait_group_read<0>();        // lane 0: the last pass's stores have read the boxes
-        pending = false;
+        // of the boxes of this pass, the stores that read them last are done
+        if (lane == 0) {
+          if (!save_z) bulk_wait_group_read<S::BOXES - 1>();
+          else if (GATED) bulk_wait_group_read<(S::BOXES > 2 ? S::BOXES - 3 : 0)>();
+          else bulk_wait_group_read<S::BOXES - 2>();
+        }
         __syncwarp();
+        uint8_t* ybox = take_box();
+        uint8_t* zbox = save_z ? take_box() : nullptr;
+        uint8_t* ubox = save_z && GATED ? take_box() : nullptr;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int cc = p * 64 + h * 32;
@@ -478,7 +488,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
               add_bias(v, zcol);
               if constexpr (GATED) add_bias(reinterpret_cast<uint32_t(&)[32]>(u), zcol + LBN / 2);
             }
-            if (la.z != nullptr) {
+            if (save_z) {
               auto put = [&](const uint32_t (&x)[32], uint8_t* box) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -489,7 +499,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
                                  pack_16(__uint_as_float(x[8 * i + 6]), __uint_as_float(x[8 * i + 7]), bf16));
               };
               put(v, zbox);
-              if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), zbox + LIN_BOX);
+              if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), ubox);
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -527,18 +537,16 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
           if constexpr (CG == 2) mbar_arrive_cluster(empty_addr[acc]);
           else mbar_arrive(&c.tmem_empty[acc]);
         }
-        store_box(ybox, &tmap_o, static_cast<char*>(la.out), static_cast<long long>(la.n_out) * 2, row0, ycol, la.n_out, rows_here, lane, pending);
-        if constexpr (MODE == LIN_FORWARD) {
-          if (la.z != nullptr) {
-            const long long ldz = static_cast<long long>(la.N) * 2;
-            store_box(zbox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + p * 64, la.N, rows_here, lane, pending);
-            if constexpr (GATED)
-              store_box(zbox + LIN_BOX, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + LBN / 2 + p * 64, la.N, rows_here, lane, pending);
-          }
+        store_box(ybox, &tmap_o, static_cast<char*>(la.out), static_cast<long long>(la.n_out) * 2, row0, ycol, la.n_out, rows_here, lane);
+        if (save_z) {
+          const long long ldz = static_cast<long long>(la.N) * 2;
+          store_box(zbox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + p * 64, la.N, rows_here, lane);
+          if constexpr (GATED)
+            store_box(ubox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + LBN / 2 + p * 64, la.N, rows_here, lane);
         }
       }
     }
-    if (pending) bulk_wait_group<0>();                 // shared memory stays allocated until the stores are done
+    if (lane == 0) bulk_wait_group<0>();               // shared memory stays allocated until the stores are done
   } else {
     // ------------------------------------------------------------ ragged ends
     if constexpr (MODE == LIN_DW) {
@@ -550,19 +558,20 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         const int KB = k_blocks(g);
         blocks += KB;
         const int tail = tail_rows(g);
-        if (KB == 0 || tail == LBK) continue;
+        if (KB == 0 || tail % 16 == 0) continue;
         const int stage = (blocks - 1) % STAGES;
         const bool got = mbar_wait(&c.part_full[stage], phase >> stage & 1u, w, ST_TIMEOUT_PIPE_FULL);
         if (!__all_sync(0xffffffffu, got)) break;
         phase ^= 1u << stage;
         uint8_t* s = smem + stage * S::STAGE;
         constexpr int NBOX = S::STAGE / LIN_MN_BOX;
-        // rows [tail, 64) of every box: whole 128-byte rows, which the swizzle does not leave
-        for (int i = tid - 6 * 32; i < NBOX * (LBK - tail) * 8; i += LIN_MENDERS * 32) {
-          const int box = i / ((LBK - tail) * 8), r = i - box * (LBK - tail) * 8;
+        // the rows from tail to the end of its step, of every box: whole 128-byte rows, which the swizzle does not leave
+        const int chunks = (16 - tail % 16) * 8;
+        for (int i = tid - 6 * 32; i < NBOX * chunks; i += LIN_MENDERS * 32) {
+          const int box = i / chunks, r = i - box * chunks;
           *reinterpret_cast<uint4*>(s + box * LIN_MN_BOX + tail * 128 + r * 16) = make_uint4(0, 0, 0, 0);
         }
-        fence_proxy_async();
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           if constexpr (CG == 2) mbar_arrive_cluster(map_to_cta(&c.mended[stage], 0));
