@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <string.h>
 
+#include <atomic>
+
 namespace b200 {
 
 inline cudaLaunchAttribute chained_attribute() {
@@ -27,6 +29,17 @@ inline cudaError_t launch_chained(void (*kern)(P...), dim3 grid, dim3 block, siz
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
+// Gives a kernel leave to use `smem` bytes of dynamic shared memory, once per device (`done`: a bit per device).
+template <typename K>
+inline cudaError_t allow_shared_memory(K kern, int smem, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1ull))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
 }
 
 }  // namespace b200

@@ -728,27 +728,18 @@ static int lin_map(CUtensorMap* tm, const void* base, int elem, long long planes
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-// Sets a kernel's shared-memory limit once per device, and makes the device's context current: the thread that runs a
-// backward pass may not have met it yet, and tensor maps are encoded by the driver, which does not do so itself.
-template <typename K>
-static cudaError_t lin_configure(K kern, int smem, std::atomic<unsigned long long>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaSetDevice(dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1ull)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
-  return e;
-}
-
 template <int MODE, int CG, bool GATED>
 static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) {
   static std::atomic<unsigned long long> configured{0};
   using S = LinGeo<MODE, CG>;
   auto kern = linear_kernel<MODE, CG, GATED>;
   constexpr int smem = lin_smem<MODE, CG>();
-  const cudaError_t e = lin_configure(kern, smem, configured);
+  // The device's context becomes current: the thread that runs a backward pass may not have met it yet, and tensor maps
+  // are encoded by the driver, which does not do so itself.
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e == cudaSuccess) e = allow_shared_memory(kern, smem, configured);
   if (e != cudaSuccess) return static_cast<int>(e);
   CUtensorMap ta, tb, to, tz;
   const long long out_rows = MODE == LIN_DW ? static_cast<long long>(la.G) * la.N : la.M;

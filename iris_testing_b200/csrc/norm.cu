@@ -470,8 +470,9 @@ static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
   a.parts = norm_parts<MAXT>(a.T, threads, smem, sms);
   const dim3 grid(MAXT == 32 ? a.parts / NORM_WARP_ROWS : a.parts);
   auto kern = BACK ? norm_backward_kernel<T, VEC, VPT, MAXT> : norm_forward_kernel<T, VEC, VPT, MAXT>;
-  if (smem > 40 * 1024) {          // 48 KB, static shared memory included, need no leave
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<unsigned long long> allowed{0};
+  if (S > 0) {
+    const cudaError_t e = allow_shared_memory(kern, NORM_SLOT_BYTES, allowed);
     if (e != cudaSuccess) return e;
   }
   b200_count_launches(1);

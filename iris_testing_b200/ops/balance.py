@@ -5,6 +5,7 @@ No counterpart in the reference, which draws its router at random and never trai
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -30,6 +31,13 @@ _BACKWARD = Entry("b200_balance_backward", C.POINTER(BalanceArgs), C.c_void_p)
 _I32, _F32 = torch.int32, torch.float32
 
 
+@functools.lru_cache(maxsize=256)
+def _runs(T: int, E: int, elem: int, sms: int) -> Tuple[int, int]:
+    """(blocks, tokens of each)."""
+    tokens = -(-T // declare("b200_balance_runs", [C.c_int] * 4)(T, E, elem, sms))
+    return -(-T // tokens), tokens
+
+
 def _fill(logits, k, seq_rows, mask, coef, z, S):
     a = BalanceArgs()
     T, E = logits.shape
@@ -40,9 +48,7 @@ def _fill(logits, k, seq_rows, mask, coef, z, S):
         a.seq_rows, a.status = seq_rows.data_ptr(), launch_status(logits.device).data_ptr()
     if mask is not None:
         a.mask = mask.data_ptr()
-    runs = declare("b200_balance_runs", [C.c_int] * 4)(T, E, elem, sm_count(logits.device))
-    a.run_tokens = tokens = -(-T // runs)
-    a.runs = -(-T // tokens)
+    a.runs, a.run_tokens = _runs(T, E, elem, sm_count(logits.device))
     return a
 
 
@@ -93,7 +99,7 @@ class _Balance(torch.autograd.Function):
         logits, seq_rows, mask, keep = ctx.saved_tensors
         if dloss is None:
             return (None,) * 6
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         if keep is None:
             return (grad.zero_(),) + (None,) * 5
         k, coef, z = ctx.how

@@ -6,6 +6,7 @@ No counterpart in the reference, whose layer begins at the router and ends at th
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -112,8 +113,18 @@ def _fill(y, residual, weight, gate, kind, norm, scale, next_weight, eps, keep):
     return a
 
 
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+@functools.lru_cache(maxsize=256)
+def _parts(T: int, H: int, elem: int, aligned: int, sms: int) -> int:
+    return declare("b200_norm_parts", [C.c_int] * 5)(T, H, elem, aligned, sms)
+
+
 def _forward(y, residual, weight, gate, kind, norm, scale, next_weight, eps, save):
-    h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    h = _new(y)
     n = None if next_weight is None else torch.empty_like(h)
     T = y.numel() // y.shape[-1]
     stats = torch.empty((2, T), dtype=_F32, device=y.device) if save else None
@@ -136,7 +147,7 @@ def _backward(saved, kind, norm, scale, eps, need, dh, dn):
     """Gradients of (y, residual, weight, gate, next_weight), None where ``need`` says so."""
     y, residual, weight, gate, next_weight, stats = saved
     like = (y, residual, weight, gate, next_weight)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n and t is not None else None for t, n in zip(like, need)]
+    grads = [_new(t) if n and t is not None else None for t, n in zip(like, need)]
     T = y.numel() // y.shape[-1]
     if T == 0 or (dh is None and dn is None):
         return [None if g is None else g.zero_() for g in grads]
@@ -160,8 +171,7 @@ def _backward(saved, kind, norm, scale, eps, need, dh, dn):
     a.r2 = p + 4 * T
     sms = sm_count(y.device)
     if a.dw or a.dw2 or (a.dgate and kind == GATE_CHANNEL):
-        parts = declare("b200_norm_parts", [C.c_int] * 5)(T, a.H, a.elem, a.aligned, sms)
-        partial = torch.empty((2, parts, a.H), dtype=_F32, device=y.device)
+        partial = torch.empty(2 * _parts(T, a.H, a.elem, a.aligned, sms) * a.H, dtype=_F32, device=y.device)
         a.partial = partial.data_ptr()
     with on_device(y):
         _BACKWARD(a, sms, stream_ptr(y))
