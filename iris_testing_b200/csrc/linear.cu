@@ -5,7 +5,10 @@
 //   dX        dx_g = dz_g W_g                                    dz = dy act'(z), [M, N]
 //   dW        dW_g = dz_g^T x_g                                  db_g = column sums of dz_g
 //
-// One persistent kernel for the three products: warp 0 loads (TMA), warp 1 issues the MMAs, warps 2-5 drain the
+// Few rows per group: the weights are streamed once for all of them, with tokens on the narrow side of the MMA and the work
+// cut into equal shares (see linear_rows_kernel).
+//
+// Otherwise one persistent kernel for the three products: warp 0 loads (TMA), warp 1 issues the MMAs, warps 2-5 drain the
 // accumulators, warps 6-7 mend ragged ends.  An operand whose contracted dimension is contiguous is K-major
 // (x and W forward, dz for dX); the others (W for dX, both of dW) are read as they lie in memory, MN-major, in boxes of 64
 // columns x 64 contracted rows, so that nothing is ever transposed in memory.
@@ -48,6 +51,7 @@ typedef struct b200_linear_args {
   int act;                  // LinearAct
   int pair;                 // two CTAs per tile (256 rows)
   int group_m;              // M-tiles per chunk (see decode_tile)
+  float* record;            // split product: scratch of b200_linear_record_floats(); null: whole tiles
 } b200_linear_args;
 
 typedef struct b200_act_grad_args {
@@ -111,7 +115,7 @@ static_assert(lin_smem<LIN_FORWARD, 1>() <= 232448 && lin_smem<LIN_FORWARD, 2>()
                   lin_smem<LIN_DW, 2>() <= 232448, "exceeds 227 KiB of shared memory per CTA");
 
 // q = 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
-__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.f + exp2_approx(-LOG2_E * v)); }
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.f + exp2_approx(__fmul_rn(-LOG2_E, v))); }
 // The same with exp(-v) q = 1 - q beside it; the exponent is held where the exponential is finite.
 __device__ __forceinline__ void sigmoid_both(float minus_v_log2e, float& q, float& rest) {
   const float e = exp2_approx(fminf(minus_v_log2e, 100.f));
@@ -119,12 +123,15 @@ __device__ __forceinline__ void sigmoid_both(float minus_v_log2e, float& q, floa
   rest = e * q;
 }
 constexpr float GELU_A = 2.f * 0.7978845608028654f, GELU_B = GELU_A * 0.044715f;    // tanh form: v * sigmoid(A v + B v^3)
+// The products are rounded before anything is added to them, so that a result does not depend on what else its kernel
+// keeps or adds.
 __device__ __forceinline__ float act_value(float v, int act) {
   if (act == ACT_RELU) return v < 0.f ? 0.f : v;
-  if (act == ACT_SILU) return v * sigmoid_f(v);
-  if (act == ACT_GELU) return v * sigmoid_f(v * fmaf(GELU_B, v * v, GELU_A));
+  if (act == ACT_SILU) return __fmul_rn(v, sigmoid_f(v));
+  if (act == ACT_GELU) return __fmul_rn(v, sigmoid_f(v * fmaf(GELU_B, v * v, GELU_A)));
   return v;
 }
+__device__ __forceinline__ float gated_value(float gate, float up) { return __fmul_rn(__fmul_rn(gate, sigmoid_f(gate)), up); }
 __device__ __forceinline__ float act_slope(float v, int act) {
   if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
   float q, rest;
@@ -147,9 +154,12 @@ __device__ __forceinline__ float2 unpack_16(uint32_t v, bool bf16) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+struct LinTables {
+  int *g_rows, *g_row_start, *g_sched_start;
+};
 // Rows and first row of every group, and its first scheduling tile (tiles per group: by its rows, or `fixed`).  One warp.
 // Returns the rows of all groups.
-__device__ __forceinline__ long long lin_scan(LinControl& c, const int* group_rows, int G, int M, int lane, int tile_rows, int fixed) {
+__device__ __forceinline__ long long lin_scan(const LinTables& c, const int* group_rows, int G, int M, int lane, int tile_rows, int fixed) {
   long long carry = 0;
   int tcarry = 0;
   for (int base = 0; base < G; base += 32) {
@@ -254,7 +264,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   }
   __syncthreads();                      // abort_flag is set below
   if (warp == 0) {
-    const long long rows = lin_scan(c, la.group_rows, G, la.M, lane, S::TM, MODE == LIN_DW ? (la.N + S::TM - 1) / S::TM : 0);
+    const LinTables tables{c.g_rows, c.g_row_start, c.g_sched_start};
+    const long long rows = lin_scan(tables, la.group_rows, G, la.M, lane, S::TM, MODE == LIN_DW ? (la.N + S::TM - 1) / S::TM : 0);
     // more rows than the buffers hold: nothing is computed, the host reads the status
     if (lane == 0 && rows > la.M) {
       report_status(w.status, ST_OVERFLOW);
@@ -504,7 +515,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float f = __uint_as_float(v[i]);
-              if constexpr (GATED) v[i] = __float_as_uint(f * sigmoid_f(f) * __uint_as_float(u[i]));
+              if constexpr (GATED) v[i] = __float_as_uint(gated_value(f, __uint_as_float(u[i])));
               else v[i] = __float_as_uint(act_value(f, la.act));
             }
             if (la.res != nullptr && row_ok) {
@@ -698,6 +709,327 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const b200_act_grad_args
   }
 }
 
+// ----------------------------------------------------------------------------
+// Fewer tiles than SMs: the contracted dimension is split.  A tile is 128 features (rows of the MMA) x TT tokens (its
+// columns); the blocks of 64 contracted elements of all tiles are one list, cut into equal runs, one per CTA, whatever the
+// number of tiles.  With few tokens the time is that of reading the weights, and every SM reads as many as any other.  A
+// run ends inside a tile as a rule: a CTA leaves its fp32 sums of each tile it touched in record CTA + tile (both only ever
+// advance, so no two share one), and linear_join_kernel adds a tile's records in their order and does the epilogue.  The
+// same inputs give the same bits.  Gated: a tile is 64 gate rows and their 64 up rows.  dW (dense only: rows behind the
+// last come as zeros) takes x's columns for features and dz's for tokens.
+// Measured, one token: 28672 x 4096 gated weights 40 us (5.8 TB/s), 4096 x 14336 23 us; 112 and 16 tiles of 256 columns
+// took 58 and 115.
+// ----------------------------------------------------------------------------
+constexpr int ROWS_FEATURES = 128;
+constexpr int ROWS_THREADS = 192;
+constexpr int ROWS_LEAST = 4;            // blocks of a run at least: a record costs as much as reading one
+template <int TT>
+struct RowsGeo {
+  static constexpr int STAGE = ROWS_FEATURES * LBK * 2 + TT * LBK * 2;
+  static constexpr int STAGES = TT <= 32 ? 5 : TT == 64 ? 4 : TT == 128 ? 6 : 4;
+  static constexpr int PER_SM = TT <= 64 ? 2 : 1;
+  static constexpr int ACC = TT < 64 ? 64 : TT;          // TMEM columns of an accumulator; there are two
+};
+static int rows_per_sm(int TT) { return TT <= 64 ? 2 : 1; }
+struct __align__(16) RowsControl {
+  uint64_t full[6], empty[6], tmem_full[2], tmem_empty[2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int g_rows[B200_MAX_GROUPS];
+  int g_row_start[B200_MAX_GROUPS + 1];
+  int g_sched_start[B200_MAX_GROUPS + 1];      // token tiles
+};
+template <int TT>
+constexpr int rows_smem() { return RowsGeo<TT>::STAGES * RowsGeo<TT>::STAGE + static_cast<int>(sizeof(RowsControl)) + 1024; }
+static_assert(rows_smem<64>() <= 113 * 1024 && rows_smem<32>() <= 113 * 1024, "two CTAs per SM");
+static_assert(rows_smem<256>() <= 232448 && rows_smem<128>() <= 232448, "exceeds 227 KiB of shared memory per CTA");
+
+// Sizes of a product: features, tokens (of the one group, where there are no group sizes) and blocks of the contraction.
+__host__ __device__ __forceinline__ int rows_features(int mode, int N, int K) { return mode == LIN_FORWARD ? N : K; }
+__host__ __device__ __forceinline__ int rows_tokens(int mode, int M, int N) { return mode == LIN_DW ? N : M; }
+__host__ __device__ __forceinline__ int rows_blocks(int mode, int M, int N, int K) {
+  return ((mode == LIN_FORWARD ? K : mode == LIN_DX ? N : M) + LBK - 1) / LBK;
+}
+// Blocks of a CTA's run.
+__host__ __device__ __forceinline__ long long rows_quota(long long units, int ctas) {
+  const long long q = (units + ctas - 1) / ctas;
+  return q < ROWS_LEAST ? ROWS_LEAST : q;
+}
+
+// Tile t: its group, its feature tile and its token tile (token tiles of a feature tile one after another, so that its
+// weights are still in L2 for the next).
+__device__ __forceinline__ void rows_tile(const int* sched_start, int G, int FT, int t, int& cursor, int& ft, int& tt) {
+  while (cursor < G - 1 && t >= FT * sched_start[cursor + 1]) ++cursor;
+  const int per = sched_start[cursor + 1] - sched_start[cursor], j = t - FT * sched_start[cursor];
+  ft = j / per;
+  tt = j - ft * per;
+}
+
+template <int MODE, int TT>
+__global__ void __launch_bounds__(ROWS_THREADS, RowsGeo<TT>::PER_SM)
+linear_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const b200_linear_args la) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr int STAGES = RowsGeo<TT>::STAGES, STAGE = RowsGeo<TT>::STAGE, ACC = RowsGeo<TT>::ACC;
+  RowsControl& c = *reinterpret_cast<RowsControl*>(smem + STAGES * STAGE);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = la.G;
+  const int features = rows_features(MODE, la.N, la.K), KB = rows_blocks(MODE, la.M, la.N, la.K);
+  const int FT = (features + ROWS_FEATURES - 1) / ROWS_FEATURES;
+  const bool gated = MODE == LIN_FORWARD && la.act == ACT_SILU_GATE;
+  const bool bf16 = la.elem == ELEM_BF16;
+  WaitCtx w;
+  w.abort_flag = &c.abort_flag;
+  w.status = la.status;
+  w.budget_ns = la.wait_budget_ns;
+  if (tid == 0) {
+    c.abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&c.full[s], 1);
+      mbar_init(&c.empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&c.tmem_full[a], 1);
+      mbar_init(&c.tmem_empty[a], 128);
+    }
+    mbar_init(&c.drain, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(&c.tmem_base, 2 * ACC);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  chain_release();
+  if (warp == 0) {
+    LinTables tables{c.g_rows, c.g_row_start, c.g_sched_start};
+    const long long rows = lin_scan(tables, la.group_rows, G, rows_tokens(MODE, la.M, la.N), lane, TT, 0);
+    if (lane == 0 && rows > rows_tokens(MODE, la.M, la.N)) {
+      report_status(w.status, ST_OVERFLOW);
+      if (w.status != nullptr) atomicMax(w.status + 1, c.g_row_start[G]);
+      c.abort_flag = 1;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = c.tmem_base;
+  const bool overflow = c.abort_flag != 0;
+  const long long units = overflow ? 0 : static_cast<long long>(c.g_sched_start[G]) * FT * KB;
+  const long long quota = rows_quota(units, gridDim.x);
+  const long long u0 = min(units, quota * blockIdx.x), u1 = min(units, u0 + quota);
+  __syncthreads();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int cursor = 0, stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long u = u0; ok && u < u1;) {
+        const int t = static_cast<int>(u / KB), kb0 = static_cast<int>(u - static_cast<long long>(t) * KB);
+        const int kb1 = static_cast<int>(min(static_cast<long long>(KB), kb0 + (u1 - u)));
+        int ft, tt;
+        rows_tile(c.g_sched_start, G, FT, t, cursor, ft, tt);
+        const int f0 = gated ? (ft >> 1) * 256 + (ft & 1) * 64 : ft * ROWS_FEATURES, f1 = gated ? f0 + 128 : f0 + 64;
+        const int row = c.g_row_start[cursor] + tt * TT;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&c.empty[stage], phase ^ 1u, w, ST_TIMEOUT_PIPE_EMPTY)) { ok = false; break; }
+          uint8_t* sa = smem + stage * STAGE;
+          mbar_expect_tx(&c.full[stage], STAGE);
+          if constexpr (MODE == LIN_FORWARD) {
+            tma_load_2d(sa, &tmap_w, &c.full[stage], kb * LBK, cursor * la.N + f0);
+            tma_load_2d(sa + LIN_MN_BOX, &tmap_w, &c.full[stage], kb * LBK, cursor * la.N + f1);
+          } else if constexpr (MODE == LIN_DX) {
+            tma_load_3d(sa, &tmap_w, &c.full[stage], f0, kb * LBK, cursor);
+            tma_load_3d(sa + LIN_MN_BOX, &tmap_w, &c.full[stage], f1, kb * LBK, cursor);
+          } else {
+            tma_load_2d(sa, &tmap_w, &c.full[stage], f0, kb * LBK);
+            tma_load_2d(sa + LIN_MN_BOX, &tmap_w, &c.full[stage], f1, kb * LBK);
+          }
+          if constexpr (MODE == LIN_DW) {
+#pragma unroll
+            for (int i = 0; i < TT / 64; ++i) tma_load_2d(sa + (2 + i) * LIN_MN_BOX, &tmap_x, &c.full[stage], row + i * 64, kb * LBK);
+          } else {
+            tma_load_2d(sa + 2 * LIN_MN_BOX, &tmap_x, &c.full[stage], kb * LBK, row);
+          }
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        u += kb1 - kb0;
+      }
+      int no_abort = 0;
+      WaitCtx wd = w;
+      wd.abort_flag = &no_abort;
+      for (int i = 0; i < min(issued, STAGES); ++i) {
+        int s = stage - 1 - i;
+        uint32_t ph = phase;
+        if (s < 0) { s += STAGES; ph ^= 1u; }
+        mbar_wait(&c.full[s], ph, wd, ST_TIMEOUT_DRAIN);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr bool A_MN = MODE != LIN_FORWARD, B_MN = MODE == LIN_DW;
+      const uint32_t idesc = make_idesc_16bit(ROWS_FEATURES, TT, bf16, A_MN, B_MN);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long u = u0; ok && u < u1; ++it) {
+        const int kb0 = static_cast<int>(u % KB), n = static_cast<int>(min(static_cast<long long>(KB - kb0), u1 - u));
+        const int acc = it & 1;
+        if (!mbar_wait(&c.tmem_empty[acc], ((it >> 1) & 1) ^ 1u, w, ST_TIMEOUT_TMEM_EMPTY)) break;
+        tc_fence_after_sync();
+        for (int i = 0; i < n; ++i) {
+          if (!mbar_wait(&c.full[stage], phase, w, ST_TIMEOUT_PIPE_FULL)) { ok = false; break; }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * STAGE);
+          const uint64_t ad = A_MN ? make_smem_desc_mn_sw128(sa, LIN_MN_BOX) : make_smem_desc_sw128(sa);
+          const uint64_t bd = B_MN ? make_smem_desc_mn_sw128(sa + 2 * LIN_MN_BOX, LIN_MN_BOX) : make_smem_desc_sw128(sa + 2 * LIN_MN_BOX);
+          constexpr int ASTEP = A_MN ? 2048 / 16 : 2, BSTEP = B_MN ? 2048 / 16 : 2;
+#pragma unroll
+          for (int k = 0; k < LBK / 16; ++k) umma_bf16_ss(tmem_base + acc * ACC, ad + ASTEP * k, bd + BSTEP * k, idesc, (i | k) != 0 ? 1u : 0u);
+          umma_commit(&c.empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit(&c.tmem_full[acc]);
+        u += n;
+      }
+      umma_commit(&c.drain);
+      int no_abort = 0;
+      WaitCtx wd = w;
+      wd.abort_flag = &no_abort;
+      mbar_wait(&c.drain, 0, wd, ST_TIMEOUT_DRAIN);
+    }
+  } else {
+    const int q = warp & 3;
+    int cursor = 0, it = 0;
+    for (long long u = u0; u < u1; ++it) {
+      const int t = static_cast<int>(u / KB), kb0 = static_cast<int>(u - static_cast<long long>(t) * KB);
+      u += min(static_cast<long long>(KB - kb0), u1 - u);
+      int ft, tt;
+      rows_tile(c.g_sched_start, G, FT, t, cursor, ft, tt);
+      const int tokens = min(TT, c.g_rows[cursor] - tt * TT), acc = it & 1;
+      const bool got = mbar_wait(&c.tmem_full[acc], (it >> 1) & 1, w, ST_TIMEOUT_TMEM_FULL);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after_sync();
+      float* rec = la.record + (static_cast<size_t>(blockIdx.x) + t) * (ROWS_FEATURES * TT) + q * 32 + lane;
+#pragma unroll 1
+      for (int h = 0; h < TT; h += 16) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * ACC + h, v);
+        tmem_ld_wait();
+        if (h + 16 >= TT) {
+          tc_fence_before_sync();
+          mbar_arrive(&c.tmem_empty[acc]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (h + i < tokens) rec[(h + i) * ROWS_FEATURES] = __uint_as_float(v[i]);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 2 * ACC);
+  }
+}
+
+// Adds a tile's records and does the epilogue: a block takes four of a tile's 4 * `quads` tokens, a thread a feature of each
+// (gated: an output of two of them).
+constexpr int JOIN_TOKENS = 4;
+template <int MODE, int TT, typename T>
+__global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_linear_args la, int ctas, int quads) {
+  __shared__ int g_rows[B200_MAX_GROUPS], g_row_start[B200_MAX_GROUPS + 1], g_sched_start[B200_MAX_GROUPS + 1];
+  __shared__ int too_many;
+  const int tid = threadIdx.x;
+  const int features = rows_features(MODE, la.N, la.K), KB = rows_blocks(MODE, la.M, la.N, la.K);
+  const int FT = (features + ROWS_FEATURES - 1) / ROWS_FEATURES;
+  chain_wait();
+  if (tid < 32) {
+    LinTables tables{g_rows, g_row_start, g_sched_start};
+    const long long rows = lin_scan(tables, la.group_rows, la.G, rows_tokens(MODE, la.M, la.N), tid, TT, 0);
+    if (tid == 0) too_many = rows > rows_tokens(MODE, la.M, la.N);
+  }
+  __syncthreads();
+  if (too_many) return;
+  const int tiles = g_sched_start[la.G] * FT;
+  const long long units = static_cast<long long>(tiles) * KB, quota = rows_quota(units, ctas);
+  const bool gated = MODE == LIN_FORWARD && la.act == ACT_SILU_GATE;
+  const long long jobs = static_cast<long long>(tiles) * quads;
+  int cursor = 0;
+  for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const int t = static_cast<int>(job / quads), k0 = static_cast<int>(job % quads) * JOIN_TOKENS;
+    int ft, tt;
+    rows_tile(g_sched_start, la.G, FT, t, cursor, ft, tt);
+    const int g = cursor, tokens = min(TT, g_rows[g] - tt * TT) - k0;      // of this block, up to JOIN_TOKENS
+    if (tokens <= 0) continue;
+    const size_t row0 = static_cast<size_t>(g_row_start[g]) + tt * TT + k0;
+    const int first = static_cast<int>(static_cast<long long>(t) * KB / quota), last = static_cast<int>((static_cast<long long>(t + 1) * KB - 1) / quota);
+    // this thread's four sums: feature f of tokens k, k + step, ...; gated: gate and up of two tokens
+    const int f = gated ? tid & 63 : tid, k = gated ? tid >> 6 : 0, step = gated ? 2 : 1;
+    const float* rec = la.record + (static_cast<size_t>(first) + t) * (ROWS_FEATURES * TT) + static_cast<size_t>(k0 + k) * ROWS_FEATURES + f;
+    auto at = [&](int j) { return gated ? (j >> 1) * 2 * ROWS_FEATURES + (j & 1) * 64 : j * ROWS_FEATURES; };
+    bool have[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) have[j] = k + (gated ? j >> 1 : j) * step < tokens;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = first; i <= last; ++i) {
+      const float* r = rec + static_cast<size_t>(i - first) * (ROWS_FEATURES * TT);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += r[at(j)];      // tokens that are none read what lies in the record, and end below
+    }
+    T* y = static_cast<T*>(la.out);
+    if (gated) {
+      const int zc = (ft >> 1) * 256 + (ft & 1) * 64 + f, yc = ft * 64 + f;
+      if (la.bias != nullptr) {
+        const T* b = static_cast<const T*>(la.bias) + static_cast<size_t>(g) * la.N + zc;
+        const float bg = to_f32(b[0]), bu = to_f32(b[128]);
+        v[0] += bg; v[1] += bu; v[2] += bg; v[3] += bu;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (!have[2 * j]) continue;
+        const size_t row = row0 + k + 2 * j;
+        if (la.z != nullptr) {
+          static_cast<T*>(la.z)[row * la.N + zc] = from_f32<T>(v[2 * j]);
+          static_cast<T*>(la.z)[row * la.N + zc + 128] = from_f32<T>(v[2 * j + 1]);
+        }
+        float o = gated_value(v[2 * j], v[2 * j + 1]);
+        if (la.res != nullptr) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + yc]);
+        y[row * la.n_out + yc] = from_f32<T>(o);
+      }
+    } else {
+      const int c = ft * ROWS_FEATURES + tid;
+      if (c >= features) continue;
+      const float b = MODE == LIN_FORWARD && la.bias != nullptr ? to_f32(static_cast<const T*>(la.bias)[static_cast<size_t>(g) * la.N + c]) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!have[j]) continue;
+        const size_t row = row0 + j;
+        float o = v[j];
+        if constexpr (MODE == LIN_FORWARD) {
+          o += b;
+          if (la.z != nullptr) static_cast<T*>(la.z)[row * la.N + c] = from_f32<T>(o);
+          o = act_value(o, la.act);
+          if (la.res != nullptr) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + c]);
+        }
+        y[row * la.n_out + c] = from_f32<T>(o);
+      }
+    }
+  }
+  // rows of the buffer behind the last group
+  const long long begin = static_cast<long long>(g_row_start[la.G]) * la.n_out / 8, end = static_cast<long long>(rows_tokens(MODE, la.M, la.N)) * la.n_out / 8;
+  uint4* out = reinterpret_cast<uint4*>(la.out);
+  for (long long i = begin + static_cast<long long>(blockIdx.x) * ROWS_FEATURES + tid; i < end; i += static_cast<long long>(gridDim.x) * ROWS_FEATURES)
+    out[i] = make_uint4(0, 0, 0, 0);
+}
+
 // ------------------------------------------------------------------ host side
 typedef CUresult (*LinEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -771,6 +1103,58 @@ static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) 
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tz, la));
 }
 
+// Tokens of a tile: as few as hold an average group.
+static int rows_tile_tokens(int mode, int M, int N, int G) {
+  const long long n = rows_tokens(mode, M, N), g = G;
+  if (mode == LIN_DW) return n <= 64 ? 64 : n <= 128 ? 128 : 256;      // whole boxes of 64
+  return n <= 16 * g ? 16 : n <= 32 * g ? 32 : n <= 64 * g ? 64 : n <= 128 * g ? 128 : 256;
+}
+static long long rows_tiles_most(int mode, int M, int N, int K, int G) {
+  const int n = rows_tokens(mode, M, N), TT = rows_tile_tokens(mode, M, N, G);
+  const long long token_tiles = (static_cast<long long>(n) + TT - 1) / TT + (G > 1 ? (G < n ? G : n) : 0);   // each group may leave one partly filled
+  return token_tiles * ((rows_features(mode, N, K) + ROWS_FEATURES - 1) / ROWS_FEATURES);
+}
+
+template <int MODE, int TT>
+static int linear_rows_launch(const b200_linear_args& la, int sms, cudaStream_t st) {
+  static std::atomic<unsigned long long> configured{0};
+  auto kern = linear_rows_kernel<MODE, TT>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);       // as in linear_launch
+  if (e == cudaSuccess) e = allow_shared_memory(kern, rows_smem<TT>(), configured);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  CUtensorMap tw, tx;
+  int r = MODE == LIN_FORWARD ? lin_map(&tw, la.b, la.elem, 0, static_cast<long long>(la.G) * la.N, la.K, 64)
+          : MODE == LIN_DX    ? lin_map(&tw, la.b, la.elem, la.G, la.N, la.K, LBK)
+                              : lin_map(&tw, la.b, la.elem, 0, la.M, la.K, LBK);
+  if (r == 0) r = lin_map(&tx, la.a, la.elem, 0, la.M, MODE == LIN_FORWARD ? la.K : la.N, MODE == LIN_DW ? LBK : TT);
+  if (r != 0) return r;
+  const int ctas = RowsGeo<TT>::PER_SM * sms;
+  b200_count_launches(2);
+  kern<<<ctas, ROWS_THREADS, rows_smem<TT>(), st>>>(tw, tx, la);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int tokens = rows_tokens(MODE, la.M, la.N);
+  const int quads = ((tokens < TT ? tokens : TT) + JOIN_TOKENS - 1) / JOIN_TOKENS;      // no tile has more tokens than there are
+  const long long jobs = rows_tiles_most(MODE, la.M, la.N, la.K, la.G) * quads;
+  const dim3 grid(static_cast<unsigned>(jobs < 16ll * sms ? jobs : 16ll * sms));
+  e = la.elem == ELEM_BF16 ? launch_chained(linear_join_kernel<MODE, TT, __nv_bfloat16>, grid, dim3(ROWS_FEATURES), 0, st, la, ctas, quads)
+                           : launch_chained(linear_join_kernel<MODE, TT, __half>, grid, dim3(ROWS_FEATURES), 0, st, la, ctas, quads);
+  return static_cast<int>(e);
+}
+template <int MODE>
+static int linear_rows(const b200_linear_args& la, int sms, cudaStream_t st) {
+  const int TT = rows_tile_tokens(MODE, la.M, la.N, la.G);
+  if constexpr (MODE != LIN_DW) {
+    if (TT == 16) return linear_rows_launch<MODE, 16>(la, sms, st);
+    if (TT == 32) return linear_rows_launch<MODE, 32>(la, sms, st);
+  }
+  if (TT == 64) return linear_rows_launch<MODE, 64>(la, sms, st);
+  if (TT == 128) return linear_rows_launch<MODE, 128>(la, sms, st);
+  return linear_rows_launch<MODE, 256>(la, sms, st);
+}
+
 template <typename T>
 static cudaError_t act_grad_launch(const b200_act_grad_args& a, cudaStream_t st) {
   const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
@@ -796,6 +1180,11 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   if (gated && la.N % 256 != 0) return -13;
   if (la.n_out != (la.mode != LIN_FORWARD ? la.K : gated ? la.N / 2 : la.N)) return -14;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (la.record != nullptr) {
+    if (la.mode == LIN_FORWARD) return linear_rows<LIN_FORWARD>(la, ctas, st);
+    if (la.mode == LIN_DX) return linear_rows<LIN_DX>(la, ctas, st);
+    return la.mode == LIN_DW && la.group_rows == nullptr ? linear_rows<LIN_DW>(la, ctas, st) : -16;
+  }
   // rows of tiles that share a stretch of the weights while it is in L2: about 48 MB of the row operand, at most 16 tiles
   const long long tile_bytes = static_cast<long long>(la.pair ? 2 * LBM : LBM) * (la.mode == LIN_DX ? la.N : la.K) * 2;
   const long long gm = (48ll << 20) / tile_bytes;
@@ -808,6 +1197,13 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
     case LIN_DW: return la.pair ? linear_launch<LIN_DW, 2, false>(la, ctas, st) : linear_launch<LIN_DW, 1, false>(la, ctas, st);
   }
   return -15;
+}
+
+// Floats of `record` for a split product: a record per CTA and tile that a CTA's run may end in.
+long long b200_linear_record_floats(int mode, int M, int N, int K, int G, int sms) {
+  using namespace b200;
+  const int TT = rows_tile_tokens(mode, M, N, G);
+  return (rows_per_sm(TT) * sms + rows_tiles_most(mode, M, N, K, G)) * ROWS_FEATURES * TT;
 }
 
 int b200_act_grad(const b200_act_grad_args* args, void* stream) {

@@ -7,13 +7,14 @@ weight per expert over packed ragged rows, with its gradients.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
 
 from .. import _native as nv
 from . import cpu_ref
-from ._common import ELEM, Entry, launch_status, on_device, require, require_device, stream_ptr, use_native
+from ._common import ELEM, Entry, declare, launch_status, on_device, require, require_device, stream_ptr, use_native
 from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
@@ -24,7 +25,8 @@ _BIAS_CHUNK = 64          # rows whose sum is one record of the bias gradient
 class LinearArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("a", "b", "out", "z", "bias", "res", "group_rows", "status")] \
         + [("wait_budget_ns", C.c_ulonglong)] \
-        + [(n, C.c_int) for n in ("mode", "G", "M", "N", "K", "n_out", "elem", "act", "pair", "group_m")]
+        + [(n, C.c_int) for n in ("mode", "G", "M", "N", "K", "n_out", "elem", "act", "pair", "group_m")] \
+        + [("record", C.c_void_p)]
 
 
 class ActGradArgs(C.Structure):
@@ -50,6 +52,29 @@ def _pairs(mode: int, M: int, N: int, K: int, G: int) -> bool:
     return pairs_pay(M / G)
 
 
+def _splits(mode: int, M: int, N: int, K: int, G: int, grouped: bool, sms: int) -> bool:
+    """Whether the contracted dimension is split over the SMs: where whole tiles would leave most of them without work for
+    long, or have a few of them read all the weights for a few tokens.
+
+    Measured on one B200 (split / whole tiles, us, launches included), bf16, x [M, K], w [N, K]: forward of 4096 x 4096 40 / 44
+    at 256 rows (32 SMs have a tile, 64 blocks each) and 50 / 46 at 512; of 4096 x 14336 (224 blocks) 97 / 101 at 512 rows;
+    of 256 x 2048 (32 blocks) 25 / 26 at 2048 rows and 31 / 26 at 4096; dW of 768 x 768 34 / 49 over 4096 rows and 29 / 24 over
+    1024.  One token of 28672 x 4096 (112 SMs) 51 / 67, 64 tokens 66 / 60.  Groups' dW ends inside a block as a
+    rule and is not split."""
+    if mode == _DW and grouped:
+        return False
+    pair = _pairs(mode, M, N, K, G)
+    rows, cols, blocks = (N, K, M) if mode == _DW else (-(-M // G), N if mode == _FORWARD else K, K if mode == _FORWARD else N)
+    blocks = -(-blocks // 64)
+    busy = G * -(-rows // (256 if pair else 128)) * -(-cols // 256) * (2 if pair else 1)
+    return busy <= min(64, blocks // 2) or (mode != _DW and busy < sms and blocks >= 16 and M <= 16 * G)
+
+
+@functools.lru_cache(maxsize=256)
+def _record_floats(mode: int, M: int, N: int, K: int, G: int, sms: int) -> int:
+    return declare("b200_linear_record_floats", [C.c_int] * 6, C.c_longlong)(mode, M, N, K, G, sms)
+
+
 def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, res=None):
     la = LinearArgs()
     la.a, la.b, la.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
@@ -64,8 +89,14 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
     la.status = launch_status(a.device).data_ptr()
     la.wait_budget_ns = 2_000_000_000
     la.mode, la.G, la.M, la.N, la.K, la.n_out = mode, G, M, N, K, out.shape[-1]
-    la.elem, la.act, la.pair = ELEM[a.dtype], act, int(_pairs(mode, M, N, K, G))
-    _PRODUCT(la, sm_count(a.device), stream_ptr(a))
+    la.elem, la.act = ELEM[a.dtype], act
+    sms = sm_count(a.device)
+    if _splits(mode, M, N, K, G, group_rows is not None, sms):
+        record = torch.empty(_record_floats(mode, M, N, K, G, sms), dtype=torch.float32, device=a.device)
+        la.record = record.data_ptr()
+    else:
+        la.pair = _pairs(mode, M, N, K, G)
+    _PRODUCT(la, sms, stream_ptr(a))
 
 
 def _forward(x, w, bias, residual, group_rows, act, save):

@@ -189,12 +189,15 @@ def test_refusals():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("pair", [False, True, None])
 @pytest.mark.parametrize("rows,N,K", [([64], 256, 64), ([128], 256, 128), ([1], 8, 8), ([300], 264, 136), ([1000], 512, 1024),
                                       ([63, 65, 1, 0, 200], 264, 136), ([0, 0, 5], 24, 40), ([0, 128, 64, 256, 0], 256, 512),
-                                      ([37] * 16, 1408, 256)])
+                                      ([37] * 16, 1408, 256), ([5000], 72, 200), ([700], 40, 4096)])
 def test_plain_products(rows, N, K, pair, monkeypatch):
-    monkeypatch.setattr(importlib.import_module("iris_testing_b200.ops.linear"), "_pairs", lambda *a: pair)
+    """Each way to cut the work, whatever the rule would take (None: split along the contraction)."""
+    mod = importlib.import_module("iris_testing_b200.ops.linear")
+    monkeypatch.setattr(mod, "_pairs", lambda *a: bool(pair))
+    monkeypatch.setattr(mod, "_splits", lambda mode, M, N, K, G, grouped, sms: pair is None and not (grouped and mode == 2))
     x, w, b, r, dy = inputs(rows, N, K, torch.bfloat16, None, False, False, "cuda", slack=9 if len(rows) > 1 else 0)
     check(x, w, b, r, dy, None, rows, dense=len(rows) == 1)
 
