@@ -211,10 +211,13 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     require(K % 8 == 0 and N % 8 == 0, "K and N must be multiples of 8")
     require(x.numel() // K < 2 ** 31 and G * N < 2 ** 31, "too many rows")
     require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)
-    x2 = _plain(x.reshape(-1, K))
-    r2 = None if residual is None else _plain(residual.reshape(-1, n_out))
-    w, b = _plain(w_kmajor), _plain(bias)
+    flat = len(shape) == 2                   # no views, which autograd would have to pass through
+    x2 = _plain(x if flat else x.reshape(-1, K))
+    r2 = residual if residual is None or flat else residual.reshape(-1, n_out)
+    w, b, r2 = _plain(w_kmajor), _plain(bias), _plain(r2)
     rows = None if group_rows is None else group_rows.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_kmajor, bias, residual)):
-        return _Linear.apply(x2, w, b, r2, rows, act).view(shape)
-    return _forward(x2, w, b, r2, rows, act, False)[0].view(shape)
+        y = _Linear.apply(x2, w, b, r2, rows, act)
+    else:
+        y, _ = _forward(x2, w, b, r2, rows, act, False)
+    return y if flat else y.view(shape)
