@@ -463,6 +463,7 @@ int b200_balance_runs(int T, int E, int elem, int sms) {
   return static_cast<int>(runs < T ? runs : T);
 }
 
+int b200_balance_max_experts() { return b200::BAL_MAX_E; }
 int b200_abi_size_balance_args() { return static_cast<int>(sizeof(b200_balance_args)); }
 
 }  // extern "C"

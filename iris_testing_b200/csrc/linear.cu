@@ -706,23 +706,28 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
   }
 }
 
+// A warp takes 32 columns and an eighth of a group's records; the eight sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(256) bias_grad_kernel(const b200_act_grad_args a) {
+  __shared__ float share[8][33];
   chain_wait();
-  const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  const int g = blockIdx.y, lane = threadIdx.x & 31, s = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   long long start = 0;
   for (int i = 0; i < g; ++i) start += max(0, a.group_rows[i]);
   const long long rows = a.group_rows != nullptr ? max(0, a.group_rows[g]) : a.M;
   const long long end = min(static_cast<long long>(a.M), start + rows);
   float v = 0.f;
-  if (c < a.N) {
-    if (end > start) {
-      const long long last = (end - 1) / a.chunk_rows;
-#pragma unroll 8
-      for (long long k = start / a.chunk_rows; k <= last; ++k) v += a.record[(static_cast<size_t>(k) + g) * a.N + c];
-    }
-    static_cast<T*>(a.dbias)[static_cast<size_t>(g) * a.N + c] = from_f32<T>(v);
+  if (c < a.N && end > start) {
+    const long long last = (end - 1) / a.chunk_rows;
+#pragma unroll 4
+    for (long long k = start / a.chunk_rows + s; k <= last; k += 8) v += a.record[(static_cast<size_t>(k) + g) * a.N + c];
   }
+  share[s][lane] = v;
+  __syncthreads();
+  if (s != 0 || c >= a.N) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v += share[i][lane];
+  static_cast<T*>(a.dbias)[static_cast<size_t>(g) * a.N + c] = from_f32<T>(v);
 }
 
 // ----------------------------------------------------------------------------
@@ -1191,6 +1196,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   if (args == nullptr || args->G < 1 || args->G > B200_MAX_GROUPS || args->M < 1 || args->N < 1 || args->K < 1 || ctas < 2) return -10;
   b200_linear_args la = *args;
   if (la.N % 8 != 0 || la.K % 8 != 0 || (la.elem != ELEM_BF16 && la.elem != ELEM_F16)) return -11;
+  if (la.mode < LIN_FORWARD || la.mode > LIN_DW) return -15;
   if ((la.group_rows == nullptr && la.G != 1) || static_cast<long long>(la.G) * la.N > 0x7fffffffll) return -12;
   const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
   if (gated && la.N % 256 != 0) return -13;
@@ -1235,7 +1241,7 @@ int b200_act_grad(const b200_act_grad_args* args, void* stream) {
   const cudaError_t launched = a.elem == ELEM_BF16 ? act_grad_launch<__nv_bfloat16>(a, st) : act_grad_launch<__half>(a, st);
   if (launched != cudaSuccess || a.dbias == nullptr) return static_cast<int>(launched);
   b200_count_launches(1);
-  const dim3 fin((a.N + 255) / 256, a.G);
+  const dim3 fin((a.N + 31) / 32, a.G);
   cudaError_t e;
   if (a.elem == ELEM_BF16) e = launch_chained(bias_grad_kernel<__nv_bfloat16>, fin, dim3(256), 0, st, a);
   else e = launch_chained(bias_grad_kernel<__half>, fin, dim3(256), 0, st, a);

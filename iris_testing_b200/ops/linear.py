@@ -19,7 +19,13 @@ from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
 _FORWARD, _DX, _DW = 0, 1, 2
-_BIAS_CHUNK = 64          # rows whose sum is one record of the bias gradient
+
+
+def _run_rows(M: int, n_out: int) -> int:
+    """Rows that a thread of the activation's gradient goes down: as many as leave 16 blocks for every SM, so that enough
+    loads are under way (64 / 32 rows: 4000 x 14336 77 / 70 us, gated 65536 x 2816 177 / 159)."""
+    blocks = -(-n_out // 1024)
+    return 64 if M * blocks >= 64 * 2368 else 32 if M * blocks >= 32 * 2368 else 16
 
 
 class LinearArgs(C.Structure):
@@ -136,7 +142,8 @@ def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
             a.dres = dres.data_ptr() if own_dres else None
             a.G, a.M, a.N, a.n_out, a.elem, a.act = G, M, N, dy.shape[1], ELEM[dt], act
             a.group_rows = None if group_rows is None else group_rows.data_ptr()
-            a.chunk_rows, a.chunks = _BIAS_CHUNK, -(-M // _BIAS_CHUNK)
+            a.chunk_rows = run = _run_rows(M, dy.shape[1])
+            a.chunks = -(-M // run)
             if db is not None:
                 record = torch.empty((a.chunks + G, N), dtype=torch.float32, device=dev)
                 a.dbias, a.record = db.data_ptr(), record.data_ptr()
