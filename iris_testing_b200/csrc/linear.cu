@@ -118,12 +118,6 @@ static_assert(lin_smem<LIN_FORWARD, 1>() <= 232448 && lin_smem<LIN_FORWARD, 2>()
 
 // q = 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
 __device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.f + exp2_approx(__fmul_rn(-LOG2_E, v))); }
-// The same with exp(-v) q = 1 - q beside it; the exponent is held where the exponential is finite.
-__device__ __forceinline__ void sigmoid_both(float minus_v_log2e, float& q, float& rest) {
-  const float e = exp2_approx(fminf(minus_v_log2e, 100.f));
-  q = rcp_approx(1.f + e);
-  rest = e * q;
-}
 constexpr float GELU_A = 2.f * 0.7978845608028654f, GELU_B = GELU_A * 0.044715f;    // tanh form: v * sigmoid(A v + B v^3)
 // The products are rounded before anything is added to them, so that a result does not depend on what else its kernel
 // keeps or adds.
@@ -134,16 +128,14 @@ __device__ __forceinline__ float act_value(float v, int act) {
   return v;
 }
 __device__ __forceinline__ float gated_value(float gate, float up) { return __fmul_rn(__fmul_rn(gate, sigmoid_f(gate)), up); }
+// Slopes, from q and 1 - q: the difference's rounding, 2^-24, is multiplied with v only while q is not yet 1.
+__device__ __forceinline__ float silu_slope(float v, float q) { return q * fmaf(v, 1.f - q, 1.f); }
 __device__ __forceinline__ float act_slope(float v, int act) {
   if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
-  float q, rest;
-  if (act == ACT_SILU) {
-    sigmoid_both(-LOG2_E * v, q, rest);
-    return q * fmaf(v, rest, 1.f);
-  }
-  const float vv = v * v;
-  sigmoid_both(v * fmaf(-LOG2_E * GELU_B, vv, -LOG2_E * GELU_A), q, rest);
-  return q * fmaf(v * fmaf(3.f * GELU_B, vv, GELU_A), rest, 1.f);
+  if (act == ACT_SILU) return silu_slope(v, sigmoid_f(v));
+  v = v > 50.f ? 50.f : v < -50.f ? -50.f : v;         // 1 and 0 from there on, and the powers of v stay finite
+  const float vv = v * v, q = sigmoid_f(v * fmaf(GELU_B, vv, GELU_A));
+  return q * fmaf(v * fmaf(3.f * GELU_B, vv, GELU_A), 1.f - q, 1.f);
 }
 
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
@@ -671,11 +663,9 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
           unpack<T, 8>(cu, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            float q, rest;
-            sigmoid_both(-LOG2_E * v[j], q, rest);
-            const float dq = d[j] * q;
-            du[j] = dq * v[j];
-            d[j] = dq * u[j] * fmaf(v[j], rest, 1.f);
+            const float q = sigmoid_f(v[j]);
+            du[j] = d[j] * (q * v[j]);
+            d[j] *= u[j] * silu_slope(v[j], q);
             if constexpr (SUMS) sum2[j] += du[j];
           }
           store_pack<T, 8>(dz + 128, du);

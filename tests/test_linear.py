@@ -371,3 +371,39 @@ def test_refusals_on_the_gpu():
                                    group_rows=torch.zeros(129, dtype=torch.int32, device="cuda"))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ACTS)
+def test_saturated_activations(act, dtype):
+    """Far from zero the slopes are 0, 1 or the other half's value; nothing overflows on the way.  At -60, the nearest, silu is
+    60 e^-60 = 5.3e-25 off its limit and its slope 59 e^-60, twice that under an up half of 2: both below 2e-24."""
+    from iris_testing_b200 import ops
+    top = 3e38 if dtype == torch.bfloat16 else 6e4
+    far = [v for v in (60.0, 3e4, 1e13, 1e15, 1e20, 1e30, 3e38) if v <= top]
+    z = torch.tensor([s * v for v in far for s in (1, -1)], dtype=dtype, device="cuda")
+    K = 128
+    n = 2 * K if act == "silu_gate" else K
+    w = torch.zeros(n, K, dtype=dtype, device="cuda")
+    w[:K] = torch.eye(K)                     # each z reaches its own column; gated: up = 2 (through the bias)
+    b = torch.zeros(n, dtype=dtype, device="cuda")
+    if act == "silu_gate":
+        b[K:] = 2.0
+    x = torch.zeros(len(z), K, dtype=dtype, device="cuda")
+    x[torch.arange(len(z)), torch.arange(len(z))] = z
+    x.requires_grad_()
+    w.requires_grad_()
+    y = ops.linear(x, w, b, activation=act)
+    dy = torch.zeros_like(y)
+    i = torch.arange(len(z), device="cuda")
+    dy[i, i] = 1.0
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    up = 2.0 if act == "silu_gate" else 1.0
+    slope = torch.ones_like(z) if act is None else (z > 0).to(dtype)
+    if act != "silu_gate":                   # twice the largest z is infinite
+        assert bool(((y.detach()[i, i].double() - torch.where(slope > 0, z, torch.zeros_like(z)).double()).abs() <= 2e-24).all())
+    assert bool(((dx[i, i].double() - up * slope.double()).abs() <= 2e-24).all()), dx[i, i]
+    off = dx.clone()
+    off[i, i] = 0
+    assert not off.any() and torch.isfinite(dx).all()
