@@ -126,8 +126,7 @@ __device__ __forceinline__ void load_token(const b200_balance_args& a, long long
 }
 
 // One token's exponentials over the lanes that share it and the inverse of their sum.  False: it takes no part.
-// exp(l - max) is 2^(l log2 e - m) with m = max log2 e rounded once per token: the shift is the same for every expert, so
-// its rounding has no part in p, and lse is m ln 2 + log(sum).
+// exp(l - max) is 2^((l - max) log2 e): the difference comes first, so that logits next to the type's largest do not overflow.
 template <typename T, int LPT, int V, int P>
 __device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, float (&p)[V * P], float& inv, float& lse) {
   constexpr int C = V * P;
@@ -145,11 +144,10 @@ __device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, floa
 #pragma unroll
   for (int o = LPT / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const bool ok = mx > lowest<T>() && mx < CUDART_INF_F;      // no for a NaN
-  const float m = mx * LOG2_E;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    p[i] = exp2_approx(fmaf(p[i], LOG2_E, -m));
+    p[i] = exp2_approx((p[i] - mx) * LOG2_E);
     sum += p[i];
   }
 #pragma unroll
@@ -159,7 +157,7 @@ __device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, floa
     for (int i = 0; i < C; ++i) p[i] = 0.f;
   }
   inv = ok ? 1.f / sum : 0.f;
-  lse = ok ? fmaf(m, LN_2, __logf(sum)) : 0.f;
+  lse = ok ? mx + logf(sum) : 0.f;
   return ok;
 }
 
@@ -205,7 +203,10 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200
           const int e = a.idx[mine * a.k + j];
           if (e >= 0 && e < a.E) atomicAdd(cnt + e, 1);
         }
-        if (sub == 0) { zsum += lse * lse; ++tokens; }
+        if (sub == 0) {
+          if (a.z != 0.f) zsum += lse * lse;       // may be infinite, and nothing times that is not nothing
+          ++tokens;
+        }
       }
       row = next;
     }

@@ -128,7 +128,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-constexpr float LOG2_E = 1.4426950408889634f, LN_2 = 0.6931471805599453f;
+constexpr float LOG2_E = 1.4426950408889634f;
 
 // Arithmetic on the values of a pack, two at a time: d = a b + c and the like, each an fp32 operation of its own.
 __device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {

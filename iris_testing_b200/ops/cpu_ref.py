@@ -280,8 +280,10 @@ def balance_loss_ref(logits: torch.Tensor, topk_idx: torch.Tensor, balance_coef:
     prob = torch.zeros(S, E, dtype=lg.dtype).index_add(0, seq, torch.softmax(lg, 1))
     some = n_s.clamp(min=1.0)
     terms = E * (counts.to(lg.dtype) * prob).sum(1) / (k * some * some)
-    z = torch.logsumexp(lg, 1).pow(2).sum() / max(t.numel(), 1)
-    return balance_coef * terms.sum() / max(int((n_s > 0).sum()), 1) + z_coef * z, counts.to(torch.int32)
+    loss = balance_coef * terms.sum() / max(int((n_s > 0).sum()), 1)
+    if z_coef != 0:
+        loss = loss + z_coef * torch.logsumexp(lg, 1).pow(2).sum() / max(t.numel(), 1)
+    return loss, counts.to(torch.int32)
 
 
 def linear_ref(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],

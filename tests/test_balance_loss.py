@@ -147,6 +147,19 @@ def test_masked_experts_and_tokens_without_any(dtype):
     check(lg, idx, rows, mask, scale=128.0)
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_next_to_the_largest(dtype, dev):
+    """Probabilities of exactly 0, 1 and 1 / 2: no z loss, whose square overflows."""
+    g = torch.Generator().manual_seed(0)
+    lg = torch.randn(12, 8, generator=g).to(dtype)
+    lg[2, 3], lg[2, 4] = 3e38, -3e38
+    lg[5] = -3e38
+    lg[5, 1] = lg[5, 6] = -2.9e38
+    idx = torch.rand(12, 8, generator=g).topk(2, dim=1).indices.to(torch.int32)
+    check(lg.to(dev), idx.to(dev), None, None, z=0.0)
+
+
 @pytest.mark.gpu
 def test_nothing_left():
     from iris_testing_b200 import ops
