@@ -54,6 +54,8 @@ namespace b200 {
 
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_E = 1024;
+// Blocks of an SM: as many runs as these make no second, half empty round.
+constexpr int BAL_FORWARD_BLOCKS = 4, BAL_BACKWARD_BLOCKS = 3;
 
 template <typename T> __device__ __forceinline__ float lowest();
 template <> __device__ __forceinline__ float lowest<float>() { return -3.402823466e38f; }
@@ -110,7 +112,8 @@ template <> __device__ __forceinline__ float minus_infinity<float>() { return -C
 template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
 template <> __device__ __forceinline__ __half minus_infinity<__half>() { return __ushort_as_half(0xfc00); }
 
-// Loads one token's logits; minus infinity behind the last expert, and everywhere where `in` is false.
+// Loads one token's logits; minus infinity behind the last expert, and everywhere where `in` is false (a masked token's are
+// loaded all the same: waiting for the mask first would put one latency behind another).
 template <typename T, int LPT, int V, int P>
 __device__ __forceinline__ void load_token(const b200_balance_args& a, long long t, bool in, int sub, TokenRow<T, V, P>& row) {
   const T* p = static_cast<const T*>(a.logits) + t * a.ld;
@@ -128,7 +131,7 @@ __device__ __forceinline__ void load_token(const b200_balance_args& a, long long
 // One token's exponentials over the lanes that share it and the inverse of their sum.  False: it takes no part.
 // exp(l - max) is 2^((l - max) log2 e): the difference comes first, so that logits next to the type's largest do not overflow.
 template <typename T, int LPT, int V, int P>
-__device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, float (&p)[V * P], float& inv, float& lse) {
+__device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, bool take, float (&p)[V * P], float& inv, float& lse) {
   constexpr int C = V * P;
   float mx = -CUDART_INF_F;
 #pragma unroll
@@ -143,7 +146,7 @@ __device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, floa
   }
 #pragma unroll
   for (int o = LPT / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const bool ok = mx > lowest<T>() && mx < CUDART_INF_F;      // no for a NaN
+  const bool ok = take && mx > lowest<T>() && mx < CUDART_INF_F;      // no for a NaN
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
@@ -162,7 +165,7 @@ __device__ __forceinline__ bool token_softmax(const TokenRow<T, V, P>& row, floa
 }
 
 template <typename T, int LPT, int V, int P>
-__global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200_balance_args a) {
+__global__ void __launch_bounds__(BAL_THREADS, V * P <= 16 ? BAL_FORWARD_BLOCKS : 2) balance_forward_kernel(const b200_balance_args a) {
   extern __shared__ float sm[];              // [warps][E] sums of p, then int [E] counts
   __shared__ float warp_z[BAL_THREADS / 32];
   __shared__ int warp_n[BAL_THREADS / 32];
@@ -189,17 +192,25 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200
     int tokens = 0;
     long long t = pos + warp * TOK;
     TokenRow<T, V, P> row, next;
-    auto takes = [&](long long at) { return at < end && (a.mask == nullptr || a.mask[at] != 0); };
-    load_token<T, LPT, V, P>(a, t + slot, takes(t + slot), sub, row);
+    bool take = false, next_take = false;
+    int chosen = -1, next_chosen = -1;         // this lane's first copy of the token
+    auto load = [&](long long at, TokenRow<T, V, P>& r, bool& take, int& chosen) {
+      const bool in = at < end;
+      load_token<T, LPT, V, P>(a, at, in, sub, r);
+      take = in && (a.mask == nullptr || a.mask[at] != 0);
+      chosen = in && sub < a.k ? a.idx[at * a.k + sub] : -1;
+    };
+    load(t + slot, row, take, chosen);
     for (; t < end; t += WARPS * TOK) {
-      const long long mine = t + slot, after = mine + WARPS * TOK;
-      load_token<T, LPT, V, P>(a, after, takes(after), sub, next);
+      const long long mine = t + slot;
+      load(mine + WARPS * TOK, next, next_take, next_chosen);
       float p[C], inv, lse;
-      const bool ok = token_softmax<T, LPT, V, P>(row, p, inv, lse);
+      const bool ok = token_softmax<T, LPT, V, P>(row, take, p, inv, lse);
 #pragma unroll
       for (int i = 0; i < C; ++i) col[i] = fmaf(p[i], inv, col[i]);
       if (ok) {
-        for (int j = sub; j < a.k; j += LPT) {
+        if (chosen >= 0 && chosen < a.E) atomicAdd(cnt + chosen, 1);
+        for (int j = sub + LPT; j < a.k; j += LPT) {
           const int e = a.idx[mine * a.k + j];
           if (e >= 0 && e < a.E) atomicAdd(cnt + e, 1);
         }
@@ -209,6 +220,8 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_forward_kernel(const b200
         }
       }
       row = next;
+      take = next_take;
+      chosen = next_chosen;
     }
     __syncwarp();
 #pragma unroll
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(FIN_WARPS * 32) balance_finish_kernel(const b2
 }
 
 template <typename T, int LPT, int V, int P>
-__global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b200_balance_args a) {
+__global__ void __launch_bounds__(BAL_THREADS, V * P <= 16 ? BAL_BACKWARD_BLOCKS : 2) balance_backward_kernel(const b200_balance_args a) {
   constexpr int WARPS = BAL_THREADS / 32, TOK = 32 / LPT, C = V * P;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LPT, slot = lane / LPT;
   const long long t0 = static_cast<long long>(blockIdx.x) * a.run_tokens;
@@ -362,13 +375,18 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b20
     }
     long long t = pos + warp * TOK;
     TokenRow<T, V, P> row, next;
-    auto takes = [&](long long at) { return n > 0 && at < end && (a.mask == nullptr || a.mask[at] != 0); };
-    load_token<T, LPT, V, P>(a, t + slot, takes(t + slot), sub, row);
+    bool take = false, next_take = false;
+    auto load = [&](long long at, TokenRow<T, V, P>& r, bool& take) {
+      const bool in = n > 0 && at < end;
+      load_token<T, LPT, V, P>(a, at, in, sub, r);
+      take = in && (a.mask == nullptr || a.mask[at] != 0);
+    };
+    load(t + slot, row, take);
     for (; t < end; t += WARPS * TOK) {
-      const long long mine = t + slot, after = mine + WARPS * TOK;
-      load_token<T, LPT, V, P>(a, after, takes(after), sub, next);
+      const long long mine = t + slot;
+      load(mine + WARPS * TOK, next, next_take);
       float p[C], inv, lse;
-      const bool ok = token_softmax<T, LPT, V, P>(row, p, inv, lse);
+      const bool ok = token_softmax<T, LPT, V, P>(row, take, p, inv, lse);
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < C; ++i) dot = fmaf(p[i], coef[i], dot);
@@ -387,6 +405,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_kernel(const b20
         }
       }
       row = next;
+      take = next_take;
     }
     __syncwarp();
     pos = end;
@@ -455,11 +474,11 @@ extern "C" {
 int b200_balance_forward(const b200_balance_args* a, void* stream) { return b200::balance_run<false>(a, stream); }
 int b200_balance_backward(const b200_balance_args* a, void* stream) { return b200::balance_run<true>(a, stream); }
 
-// Blocks (runs of tokens) of a call: as many as fill the GPU four times over, but no shorter than 32 KB of logits (a
-// record is written and read per run).
-int b200_balance_runs(int T, int E, int elem, int sms) {
+// Blocks (runs of tokens) of a call: as many as are in work at once, but no shorter than 32 KB of logits (a record is written
+// and read per run).
+int b200_balance_runs(int T, int E, int elem, int backward, int sms) {
   const long long bytes = static_cast<long long>(T) * E * (elem == b200::ELEM_F32 ? 4 : 2);
-  const long long want = (bytes + 32767) / 32768, most = 4ll * sms;
+  const long long want = (bytes + 32767) / 32768, most = static_cast<long long>(backward ? b200::BAL_BACKWARD_BLOCKS : b200::BAL_FORWARD_BLOCKS) * sms;
   const long long runs = want < most ? want : most;
   return static_cast<int>(runs < T ? runs : T);
 }

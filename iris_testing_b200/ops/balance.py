@@ -32,13 +32,13 @@ _I32, _F32 = torch.int32, torch.float32
 
 
 @functools.lru_cache(maxsize=256)
-def _runs(T: int, E: int, elem: int, sms: int) -> Tuple[int, int]:
+def _runs(T: int, E: int, elem: int, backward: bool, sms: int) -> Tuple[int, int]:
     """(blocks, tokens of each)."""
-    tokens = -(-T // declare("b200_balance_runs", [C.c_int] * 4)(T, E, elem, sms))
+    tokens = -(-T // declare("b200_balance_runs", [C.c_int] * 5)(T, E, elem, backward, sms))
     return -(-T // tokens), tokens
 
 
-def _fill(logits, k, seq_rows, mask, coef, z, S):
+def _fill(logits, k, seq_rows, mask, coef, z, S, backward=False):
     a = BalanceArgs()
     T, E = logits.shape
     elem = ELEM[logits.dtype]
@@ -48,7 +48,7 @@ def _fill(logits, k, seq_rows, mask, coef, z, S):
         a.seq_rows, a.status = seq_rows.data_ptr(), launch_status(logits.device).data_ptr()
     if mask is not None:
         a.mask = mask.data_ptr()
-    a.runs, a.run_tokens = _runs(T, E, elem, sm_count(logits.device))
+    a.runs, a.run_tokens = _runs(T, E, elem, backward, sm_count(logits.device))
     return a
 
 
@@ -104,7 +104,7 @@ class _Balance(torch.autograd.Function):
             return (grad.zero_(),) + (None,) * 5
         k, coef, z = ctx.how
         S = 1 if seq_rows is None else seq_rows.numel()
-        a = _fill(logits, k, seq_rows, mask, coef, z, S)
+        a = _fill(logits, k, seq_rows, mask, coef, z, S, True)
         _keep(a, keep.data_ptr(), S, logits.shape[1])
         if dloss.dtype != _F32:
             dloss = dloss.float()
