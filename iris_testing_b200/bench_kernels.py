@@ -5,6 +5,9 @@
     python -m iris_testing_b200.bench_kernels plan   [--tokens 16384 --experts 8 --topk 2]
     python -m iris_testing_b200.bench_kernels layer  [--model mixtral-8x7b --tokens 16384 --graph 0]
     python -m iris_testing_b200.bench_kernels pipeline [--tokens 8192 --hidden 2048 --experts 8 --topk 2]
+    python -m iris_testing_b200.bench_kernels linear   [--groups 1 --rows 4096 --n 4096 --k 4096 --activation gelu --train 0]
+    python -m iris_testing_b200.bench_kernels norm     [--tokens 16384 --hidden 4096 --train 0]
+    python -m iris_testing_b200.bench_kernels balance  [--tokens 262144 --experts 128 --topk 8 --train 0]
 
 Each sub-command warms up, times ``--iters`` launches with CUDA events and prints one JSON
 line: achieved TFLOP/s or GB/s and the fraction of the measured peaks (``MEASURED_PEAKS.json``
@@ -158,6 +161,63 @@ def cmd_pipeline(a) -> dict:
                 ms=round(ms, 4), payload_mb=round(T * k * D * 2 / 1e6, 1))
 
 
+def _step(fn, leaves, grads, train: bool):
+    """``fn`` alone, or with the gradients of ``leaves``."""
+    if not train:
+        return fn
+    for t in leaves:
+        t.requires_grad_()
+
+    def both():
+        outs = fn()
+        return torch.autograd.grad(outs, leaves, grads)
+    return both
+
+
+def cmd_linear(a) -> dict:
+    from .ops import check_default_status, linear
+    dev = torch.device("cuda")
+    G, M, N, K = a.groups, a.rows, a.n, a.k
+    act = None if a.activation == "none" else a.activation
+    x = torch.randn(G * M, K, device=dev).to(torch.bfloat16)
+    w = (torch.randn((G, N, K) if G > 1 else (N, K), device=dev) * 0.02).to(torch.bfloat16)
+    rows = torch.full((G,), M, dtype=torch.int32, device=dev) if G > 1 else None
+    dy = torch.randn(G * M, N // 2 if act == "silu_gate" else N, device=dev).to(torch.bfloat16)
+    ms = time_launches(_step(lambda: linear(x, w, activation=act, group_rows=rows), [x, w], dy, a.train), a.iters)
+    check_default_status()
+    pk = peaks()
+    tf = 2.0 * G * M * N * K * (3 if a.train else 1) / ms / 1e9
+    return dict(kernel="linear" + (" forward and backward" if a.train else ""), groups=G, rows=M, N=N, K=K,
+                activation=a.activation, ms=round(ms, 4), tflops=round(tf, 1), frac_of_peak=round(tf / pk["tflops"], 3),
+                peak=pk["kind"])
+
+
+def cmd_norm(a) -> dict:
+    from .ops import post_norm
+    dev = torch.device("cuda")
+    y, res, dh, dn = (torch.randn(a.tokens, a.hidden, device=dev).to(torch.bfloat16) for _ in range(4))
+    w, gate, w2 = (torch.rand(a.hidden, device=dev) for _ in range(3))
+    ms = time_launches(_step(lambda: post_norm(y, res, w, gate, next_weight=w2), [y, res, w, gate, w2], [dh, dn], a.train),
+                       a.iters)
+    pk = peaks()
+    gbs = y.numel() * 2 * (10 if a.train else 4) / ms / 1e6
+    return dict(kernel="post_norm" + (" forward and backward" if a.train else ""), tokens=a.tokens, hidden=a.hidden,
+                ms=round(ms, 4), gbs=round(gbs, 1), frac_of_hbm=round(gbs / pk["hbm_gbs"], 3), peak=pk["kind"])
+
+
+def cmd_balance(a) -> dict:
+    from .ops import balance_loss
+    dev = torch.device("cuda")
+    lg = torch.randn(a.tokens, a.experts, device=dev)
+    idx = torch.topk(lg, a.topk, dim=1).indices.to(torch.int32)
+    one = torch.ones((), device=dev)
+    ms = time_launches(_step(lambda: balance_loss(lg, idx, z_coef=1e-3)[0], [lg], one, a.train), a.iters)
+    pk = peaks()
+    gbs = (lg.numel() * 4 * (3 if a.train else 1) + idx.numel() * 4) / ms / 1e6
+    return dict(kernel="balance_loss" + (" forward and backward" if a.train else ""), tokens=a.tokens, experts=a.experts,
+                topk=a.topk, ms=round(ms, 4), gbs=round(gbs, 1), frac_of_hbm=round(gbs / pk["hbm_gbs"], 3), peak=pk["kind"])
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -177,11 +237,22 @@ def main() -> None:
     q = sub.add_parser("pipeline")
     q.add_argument("--tokens", type=int, default=8192); q.add_argument("--hidden", type=int, default=2048)
     q.add_argument("--experts", type=int, default=8); q.add_argument("--topk", type=int, default=2)
-    for s in (g, r, p, l, q):
+    i = sub.add_parser("linear")
+    i.add_argument("--groups", type=int, default=1); i.add_argument("--rows", type=int, default=4096)
+    i.add_argument("--n", type=int, default=4096); i.add_argument("--k", type=int, default=4096)
+    i.add_argument("--activation", default="gelu"); i.add_argument("--train", type=int, default=0)
+    n = sub.add_parser("norm")
+    n.add_argument("--tokens", type=int, default=16384); n.add_argument("--hidden", type=int, default=4096)
+    n.add_argument("--train", type=int, default=0)
+    b = sub.add_parser("balance")
+    b.add_argument("--tokens", type=int, default=262144); b.add_argument("--experts", type=int, default=128)
+    b.add_argument("--topk", type=int, default=8); b.add_argument("--train", type=int, default=0)
+    for s in (g, r, p, l, q, i, n, b):
         s.add_argument("--iters", type=int, default=5)
     a = ap.parse_args()
     torch.cuda.set_device(0)
-    out = dict(gemm=cmd_gemm, router=cmd_router, plan=cmd_plan, layer=cmd_layer, pipeline=cmd_pipeline)[a.cmd](a)
+    out = dict(gemm=cmd_gemm, router=cmd_router, plan=cmd_plan, layer=cmd_layer, pipeline=cmd_pipeline,
+               linear=cmd_linear, norm=cmd_norm, balance=cmd_balance)[a.cmd](a)
     print(json.dumps(out), flush=True)
 
 
