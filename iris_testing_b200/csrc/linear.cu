@@ -1078,7 +1078,7 @@ static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) 
   auto kern = linear_kernel<MODE, CG, GATED>;
   constexpr int smem = lin_smem<MODE, CG>();
   // The device's context becomes current: the thread that runs a backward pass may not have met it yet, and tensor maps
-  // are encoded by the driver, which does not do so itself.
+  // are encoded by the CUDA driver, which does not do so itself.
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaSetDevice(dev);

@@ -10,7 +10,6 @@ from typing import Optional, Tuple
 
 import torch
 
-from .. import _native as nv
 from . import cpu_ref
 from ._common import (ELEM, Entry, declare, launch_status, on_device, require, require_device, rows_view, stream_ptr,
                       use_native)

@@ -11,7 +11,6 @@ from typing import Optional
 
 import torch
 
-from .. import _native as nv
 from . import cpu_ref
 from ._common import ELEM, Entry, declare, on_device, require, require_device, rows_view, stream_ptr, use_native
 from .expert import sm_count

@@ -310,15 +310,19 @@ def test_empty_strided_shifted_and_leading_dimensions():
 
 
 @pytest.mark.gpu
-def test_only_the_gradients_asked_for():
+@pytest.mark.parametrize("act", ["silu_gate", "gelu", None])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_only_the_gradients_asked_for(grouped, act):
     from iris_testing_b200 import ops
-    x, w, b, r, dy = inputs([50], 256, 64, torch.bfloat16, "silu_gate", True, True, "cuda")
-    leaves = [t.detach().requires_grad_() for t in (x, w[0], b[0], r)]
-    full = torch.autograd.grad(ops.linear(*leaves, activation="silu_gate"), leaves, dy)
+    rows = [20, 0, 25] if grouped else [50]
+    x, w, b, r, dy = inputs(rows, 256, 64, torch.bfloat16, act, True, True, "cuda", slack=5 if grouped else 0)
+    gr = torch.tensor(rows, dtype=torch.int32, device="cuda") if grouped else None
+    leaves = [t.detach().requires_grad_() for t in ((x, w, b, r) if grouped else (x, w[0], b[0], r))]
+    full = torch.autograd.grad(ops.linear(*leaves, activation=act, group_rows=gr), leaves, dy)
     for i in range(4):
         args = [t if j == i else t.detach() for j, t in enumerate(leaves)]
-        one, = torch.autograd.grad(ops.linear(*args, activation="silu_gate"), leaves[i], dy)
-        assert torch.equal(one, full[i])
+        one, = torch.autograd.grad(ops.linear(*args, activation=act, group_rows=gr), leaves[i], dy)
+        assert torch.equal(one, full[i]), i
 
 
 @pytest.mark.gpu

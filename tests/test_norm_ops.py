@@ -226,6 +226,23 @@ def test_zero_rows_zero_inputs_and_missing_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["channel next w32", "row next", "full next", "nonorm channel", "pre"])
+@pytest.mark.parametrize("H", [128, 1000, 2049])
+def test_only_the_gradients_asked_for(H, kind):
+    t = make(37, H, torch.bfloat16, kind, "cuda")
+    names = [n for n in ("y", "residual", "weight", "gate", "next_weight") if n in t]
+    up = [t["dn"]] if "residual" not in t else [t.get("dh"), t.get("dn")]
+
+    def grads(wanted):
+        m = {n: x.detach().requires_grad_(n in wanted) for n, x in t.items()}
+        outs = call(m, 0.5, "nonorm" not in kind)
+        return torch.autograd.grad(outs, [m[n] for n in wanted], [d for d in up if d is not None])
+    full = dict(zip(names, grads(names)))
+    for n in names:
+        assert torch.equal(grads([n])[0], full[n]), n
+
+
+@pytest.mark.gpu
 def test_infinities_stay_in_their_row():
     from iris_testing_b200 import ops
     y = torch.randn(6, 256, device="cuda")
