@@ -19,8 +19,11 @@
 // block is loaded first and multiplied third, which hides the mending (64 groups of 1023 rows: 612 us, 631 when it came last;
 // 603 for 1024 rows, which need none).
 //
-// The hidden pre-activations z are kept for the backward pass in the element type; dz is rounded to it too, since the
-// tensor cores multiply 16-bit values: two roundings of half a step each that average out over the contracted dimension.
+// The pre-activations z are kept for the backward pass as fp16 under a power of two that 32 columns of a row share, kept in a
+// byte: 11 bits of precision in fp32's range.  (Kept as bf16, they put dX and dW of a gated bf16 product 3.0e-3 off
+// instead of 2.4e-3, relative; 1.7e-3 is what rounding the result alone costs.)
+// dz is rounded to the element type, since the tensor cores multiply 16-bit values: at most half a step of each value, which
+// averages out over the contracted dimension.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,7 +44,8 @@ typedef struct b200_linear_args {
   const void* a;            // forward: x [M, K]; dX: dz [M, N]; dW: dz [M, N]
   const void* b;            // forward, dX: W [G, N, K]; dW: x [M, K]
   void* out;                // y [M, n_out]; dx [M, K]; dW [G, N, K]
-  void* z;                  // forward: [M, N] or null
+  void* z;                  // forward: fp16 [M, N] or null
+  unsigned char* zexp;      // with z: [M][ceil(N / 256) * 8], exponents of 32 columns each
   const void* bias;         // [G, N] or null
   const void* res;          // [M, n_out] or null
   const int* group_rows;    // [G] or null: one group of all M rows
@@ -58,7 +62,8 @@ typedef struct b200_linear_args {
 
 typedef struct b200_act_grad_args {
   const void* dy;           // [M, n_out]
-  const void* z;            // [M, N] or null (no activation)
+  const void* z;            // fp16 [M, N] or null (no activation)
+  const unsigned char* zexp;   // as the forward product left it
   void* dz;                 // [M, N] or null (no activation: dz is dy)
   void* dres;               // [M, n_out] or null: dy of the groups' rows, zero behind them
   void* dbias;              // [G, N] or null
@@ -137,6 +142,13 @@ __device__ __forceinline__ float act_slope(float v, int act) {
   const float vv = v * v, q = sigmoid_f(v * fmaf(GELU_B, vv, GELU_A));
   return q * fmaf(v * fmaf(3.f * GELU_B, vv, GELU_A), 1.f - q, 1.f);
 }
+
+// z in fp16 under a shared power of two: E is the largest finite magnitude's exponent (biased, 15 at least), the
+// values are scaled into [0, 2^15], where fp16 has 11 bits down to 2^-14.  Infinities and NaN stay what they are.
+__device__ __forceinline__ int shared_exponent(uint32_t largest_finite_bits) { return max(15, static_cast<int>(largest_finite_bits >> 23)); }
+__device__ __forceinline__ float z_scale(int E) { return __uint_as_float(static_cast<uint32_t>(268 - E) << 23); }      // 2^(141 - E)
+__device__ __forceinline__ float z_unscale(int E) { return __uint_as_float(static_cast<uint32_t>(E - 14) << 23); }    // 2^(E - 141)
+__device__ __forceinline__ long long zexp_pitch(int N) { return (N + 255) / 256 * 8; }
 
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
   if (bf16) return pack_bf16x2(lo, hi);
@@ -461,6 +473,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       tc_fence_after_sync();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * LBN;
       const bool row_ok = lane < rows_here;
+      unsigned long long exponents = 0;                // of this row's eight chunks of 32 columns
 #pragma unroll 1
       for (int p = 0; p < OUT_TILE / 64; ++p) {
         const int ycol = n * OUT_TILE + p * 64;        // first output column of the pass
@@ -507,17 +520,31 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
               if constexpr (GATED) add_bias(reinterpret_cast<uint32_t(&)[32]>(u), zcol + LBN / 2);
             }
             if (save_z) {
-              auto put = [&](const uint32_t (&x)[32], uint8_t* box) {
+              auto put = [&](const uint32_t (&x)[32], uint8_t* box, int col, int chunk) {
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (col + (i & ~7) < la.N) m = fmaxf(m, fabsf(__uint_as_float(x[i])));
+                if (m > 3.402823466e38f) {             // an infinity: the largest of the others
+                  m = 0.f;
+                  for (int i = 0; i < 32; ++i) {
+                    const float f = fabsf(__uint_as_float(x[i]));
+                    if (col + (i & ~7) < la.N && f <= 3.402823466e38f) m = fmaxf(m, f);
+                  }
+                }
+                const int E = shared_exponent(__float_as_uint(m));
+                const float s = z_scale(E);
+                exponents |= static_cast<unsigned long long>(E) << (8 * chunk);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                   *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
-                      make_uint4(pack_16(__uint_as_float(x[8 * i]), __uint_as_float(x[8 * i + 1]), bf16),
-                                 pack_16(__uint_as_float(x[8 * i + 2]), __uint_as_float(x[8 * i + 3]), bf16),
-                                 pack_16(__uint_as_float(x[8 * i + 4]), __uint_as_float(x[8 * i + 5]), bf16),
-                                 pack_16(__uint_as_float(x[8 * i + 6]), __uint_as_float(x[8 * i + 7]), bf16));
+                      make_uint4(pack_16(__uint_as_float(x[8 * i]) * s, __uint_as_float(x[8 * i + 1]) * s, false),
+                                 pack_16(__uint_as_float(x[8 * i + 2]) * s, __uint_as_float(x[8 * i + 3]) * s, false),
+                                 pack_16(__uint_as_float(x[8 * i + 4]) * s, __uint_as_float(x[8 * i + 5]) * s, false),
+                                 pack_16(__uint_as_float(x[8 * i + 6]) * s, __uint_as_float(x[8 * i + 7]) * s, false));
               };
-              put(v, zbox);
-              if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), ubox);
+              put(v, zbox, zcol, p * 2 + h);
+              if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), ubox, zcol + LBN / 2, 4 + p * 2 + h);
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -563,6 +590,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             store_box(ubox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + LBN / 2 + p * 64, la.N, rows_here, lane);
         }
       }
+      if (save_z && row_ok)
+        *reinterpret_cast<unsigned long long*>(la.zexp + (row0 + lane) * zexp_pitch(la.N) + n * 8) = exponents;
     }
     if (lane == 0) bulk_wait_group<0>();               // shared memory stays allocated until the stores are done
   } else {
@@ -620,6 +649,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 template <typename T, bool GATED, bool SUMS>
 __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_args a) {
   using P = Pack<T, 8>;
+  using Z = Pack<__half, 8>;
   // of the gated form, a thread's columns belong to eight columns of the gate and of the up half
   const int oc = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (oc >= a.n_out) return;
@@ -630,8 +660,10 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
   auto rows_of = [&](int i) { return a.group_rows != nullptr ? max(0, a.group_rows[i]) : a.M; };
   while (g < a.G && start + rows_of(g) <= first) start += rows_of(g++);
   const T* dy = static_cast<const T*>(a.dy) + oc;
-  const T* z = static_cast<const T*>(a.z) + zc;
+  const __half* z = static_cast<const __half*>(a.z) + zc;
   const bool active = a.z != nullptr;
+  const unsigned char* zexp = a.zexp + zc / 32;            // gated: the up half's four bytes on
+  const long long pitch = zexp_pitch(a.N);
   long long pos = first;
   for (; g < a.G && pos < r1; ++g) {
     const long long end = min(r1, start + rows_of(g));
@@ -642,25 +674,37 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] = sum2[j] = 0.f;
     }
-    P kd, kz, ku;
+    P kd;
+    Z kz, ku;
+    int ez = 141, eu = 141;
     auto load = [&](long long r) {
       kd = *reinterpret_cast<const P*>(dy + r * a.n_out);
-      if (active) kz = *reinterpret_cast<const P*>(z + r * a.N);
-      if (GATED) ku = *reinterpret_cast<const P*>(z + r * a.N + 128);
+      if (active) {
+        kz = *reinterpret_cast<const Z*>(z + r * a.N);
+        ez = zexp[r * pitch];
+      }
+      if (GATED) {
+        ku = *reinterpret_cast<const Z*>(z + r * a.N + 128);
+        eu = zexp[r * pitch + 4];
+      }
     };
     load(pos);
     for (long long r = pos; r < end; ++r) {
-      const P cd = kd, cz = kz, cu = ku;
+      const P cd = kd;
+      const Z cz = kz, cu = ku;
+      const float sz = z_unscale(ez), su = z_unscale(eu);
       if (r + 1 < end) load(r + 1);
       if (a.dres != nullptr) *reinterpret_cast<P*>(static_cast<T*>(a.dres) + r * a.n_out + oc) = cd;
       float d[8], v[8];
       unpack<T, 8>(cd, d);
       if (active) {
         T* dz = static_cast<T*>(a.dz) + r * a.N + zc;
-        unpack<T, 8>(cz, v);
+        unpack<__half, 8>(cz, v);
+        v_mul<8>(v, v, sz);
         if constexpr (GATED) {
           float u[8], du[8];
-          unpack<T, 8>(cu, u);
+          unpack<__half, 8>(cu, u);
+          v_mul<8>(u, u, su);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float q = sigmoid_f(v[j]);
@@ -953,6 +997,13 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 // Adds a tile's records and does the epilogue: a block takes four of a tile's 4 * `quads` tokens, a thread a feature of each
 // (gated: an output of two of them).
 constexpr int JOIN_TOKENS = 4;
+// z of column c, by a warp that has 32 columns of the row, those that a byte of exponents is for.
+__device__ __forceinline__ void keep_z(const b200_linear_args& la, size_t row, int c, bool in, float z) {
+  const uint32_t bits = __float_as_uint(fabsf(z));
+  const int E = shared_exponent(__reduce_max_sync(0xffffffffu, in && bits < 0x7f800000u ? bits : 0u));
+  if ((threadIdx.x & 31) == 0 && in) la.zexp[row * zexp_pitch(la.N) + c / 32] = static_cast<unsigned char>(E);
+  if (in) static_cast<__half*>(la.z)[row * la.N + c] = __float2half_rn(z * z_scale(E));
+}
 template <int MODE, int TT, typename T>
 __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_linear_args la, int ctas, int quads) {
   __shared__ int g_rows[B200_MAX_GROUPS], g_row_start[B200_MAX_GROUPS + 1], g_sched_start[B200_MAX_GROUPS + 1];
@@ -1008,8 +1059,8 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
         if (!have[2 * j]) continue;
         const size_t row = row0 + k + 2 * j;
         if (la.z != nullptr) {
-          static_cast<T*>(la.z)[row * la.N + zc] = from_f32<T>(v[2 * j]);
-          static_cast<T*>(la.z)[row * la.N + zc + 128] = from_f32<T>(v[2 * j + 1]);
+          keep_z(la, row, zc, true, v[2 * j]);
+          keep_z(la, row, zc + 128, true, v[2 * j + 1]);
         }
         float o = gated_value(v[2 * j], v[2 * j + 1]);
         if (la.res != nullptr) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + yc]);
@@ -1017,8 +1068,8 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
       }
     } else {
       const int c = ft * ROWS_FEATURES + tid;
-      if (c >= features) continue;
-      const float b = MODE == LIN_FORWARD && la.bias != nullptr ? to_f32(static_cast<const T*>(la.bias)[static_cast<size_t>(g) * la.N + c]) : 0.f;
+      const bool in = c < features;
+      const float b = MODE == LIN_FORWARD && la.bias != nullptr && in ? to_f32(static_cast<const T*>(la.bias)[static_cast<size_t>(g) * la.N + c]) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (!have[j]) continue;
@@ -1026,11 +1077,11 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
         float o = v[j];
         if constexpr (MODE == LIN_FORWARD) {
           o += b;
-          if (la.z != nullptr) static_cast<T*>(la.z)[row * la.N + c] = from_f32<T>(o);
+          if (la.z != nullptr) keep_z(la, row, c, in, o);
           o = act_value(o, la.act);
-          if (la.res != nullptr) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + c]);
+          if (la.res != nullptr && in) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + c]);
         }
-        y[row * la.n_out + c] = from_f32<T>(o);
+        if (in) y[row * la.n_out + c] = from_f32<T>(o);
       }
     }
   }
@@ -1190,6 +1241,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   if ((la.group_rows == nullptr && la.G != 1) || static_cast<long long>(la.G) * la.N > 0x7fffffffll) return -12;
   const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
   if (gated && la.N % 256 != 0) return -13;
+  if ((la.z != nullptr) != (la.zexp != nullptr)) return -17;
   if (la.n_out != (la.mode != LIN_FORWARD ? la.K : gated ? la.N / 2 : la.N)) return -14;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (la.record != nullptr) {
@@ -1226,6 +1278,7 @@ int b200_act_grad(const b200_act_grad_args* args, void* stream) {
   if (args->dbias != nullptr && args->record == nullptr) return -11;
   if ((args->act != ACT_NONE) != (args->z != nullptr) || (args->z != nullptr) != (args->dz != nullptr)) return -12;
   if (args->elem != ELEM_BF16 && args->elem != ELEM_F16) return -13;
+  if ((args->z != nullptr) != (args->zexp != nullptr)) return -14;
   const b200_act_grad_args& a = *args;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t launched = a.elem == ELEM_BF16 ? act_grad_launch<__nv_bfloat16>(a, st) : act_grad_launch<__half>(a, st);

@@ -29,14 +29,14 @@ def _run_rows(M: int, n_out: int) -> int:
 
 
 class LinearArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("a", "b", "out", "z", "bias", "res", "group_rows", "status")] \
+    _fields_ = [(n, C.c_void_p) for n in ("a", "b", "out", "z", "zexp", "bias", "res", "group_rows", "status")] \
         + [("wait_budget_ns", C.c_ulonglong)] \
         + [(n, C.c_int) for n in ("mode", "G", "M", "N", "K", "n_out", "elem", "act", "pair", "group_m")] \
         + [("record", C.c_void_p)]
 
 
 class ActGradArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "dz", "dres", "dbias", "record", "group_rows")] \
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "zexp", "dz", "dres", "dbias", "record", "group_rows")] \
         + [(n, C.c_int) for n in ("G", "M", "N", "n_out", "elem", "act", "chunks", "chunk_rows")]
 
 
@@ -87,7 +87,7 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
     la = LinearArgs()
     la.a, la.b, la.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
     if z is not None:
-        la.z = z.data_ptr()
+        la.z, la.zexp = z[0].data_ptr(), z[1].data_ptr()
     if bias is not None:
         la.bias = bias.data_ptr()
     if res is not None:
@@ -108,12 +108,16 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
 
 
 def _forward(x, w, bias, residual, group_rows, act, save):
-    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain."""
+    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain.  z is fp16 [M, N] and a byte of exponent for every
+    32 columns of a row."""
     M, K = x.shape
     G, N = (1, w.shape[0]) if w.dim() == 2 else w.shape[:2]
     n_out = N // 2 if act == 4 else N
     y = torch.empty((M, n_out), dtype=x.dtype, device=x.device)
-    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save and act else None
+    z = None
+    if save and act:
+        z = (torch.empty((M, N), dtype=torch.float16, device=x.device),
+             torch.empty((M, -(-N // 256) * 8), dtype=torch.uint8, device=x.device))
     if M > 0:
         with on_device(x):
             _product(_FORWARD, x, w, y, M, N, K, G, group_rows, act, z, bias, residual)
@@ -140,7 +144,7 @@ def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
             a = ActGradArgs()
             if slope:
                 dz = torch.empty((M, N), dtype=dt, device=dev)
-                a.z, a.dz, a.act = z.data_ptr(), dz.data_ptr(), act
+                a.z, a.zexp, a.dz, a.act = z[0].data_ptr(), z[1].data_ptr(), dz.data_ptr(), act
             a.dy = dy.data_ptr()
             a.dres = dres.data_ptr() if own_dres else None
             a.G, a.M, a.N, a.n_out, a.elem = G, M, dz.shape[1], dy.shape[1], ELEM[dt]
@@ -162,16 +166,16 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, group_rows, act):
         y, z = _forward(x, w, bias, residual, group_rows, act, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, w, z, group_rows)
+        ctx.save_for_backward(x, w, *(z or (None, None)), group_rows)
         ctx.how = (bias is not None, residual is not None, act)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, z, group_rows = ctx.saved_tensors
+        x, w, z, exponents, group_rows = ctx.saved_tensors
         has_bias, has_res, act = ctx.how
-        return (*_backward(x, w, z, has_bias, has_res, group_rows, act, ctx.needs_input_grad[:4], _plain(dy)), None, None)
+        return (*_backward(x, w, (z, exponents), has_bias, has_res, group_rows, act, ctx.needs_input_grad[:4], _plain(dy)), None, None)
 
 
 def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -187,8 +191,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     group_rows  int32 [G] on x's device: rows of each group, none allowed.  Rows of x behind the last group are not read;
                 the result and the gradients of x and residual are zero there.
 
-    All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; a backward pass keeps the
-    pre-activation and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
+    All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
+    the pre-activation is kept to 11 bits and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
     timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.  CPU tensors take
     plain PyTorch."""
     if activation not in ACTIVATIONS:

@@ -378,6 +378,34 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("act,N", [("silu", 136), ("silu_gate", 256)])
+def test_kept_pre_activations_have_11_bits(act, N, split, monkeypatch):
+    """What the forward pass keeps for the backward one, in rows of very different sizes and next to an infinity and a NaN: off by
+    half a step of 11 bits, or of the smallest normal number under the chunk's scale, 2^-24 2^-14 of its largest value's power of two."""
+    mod = importlib.import_module("iris_testing_b200.ops.linear")
+    monkeypatch.setattr(mod, "_splits", lambda *a: split)
+    M, K = 160, N
+    g = torch.Generator().manual_seed(3)
+    size = torch.exp2(torch.randint(-100, 100, (M, 1), generator=g).float()) * torch.exp2(torch.randint(-8, 1, (1, K), generator=g).float())
+    x = (torch.randn(M, K, generator=g) * size).to("cuda", torch.bfloat16)
+    w = torch.eye(K).to("cuda", torch.bfloat16)                   # z is x + b, exact but for one fp32 rounding
+    b = (torch.randn(N, generator=g) * 2.0 ** -9).to("cuda", torch.bfloat16)
+    b[5], b[70] = float("inf"), float("nan")
+    x[11] = 0
+    x[12, 40:72] = 2.0 ** -126                                    # next to nothing, under a bias
+    _, (z, e) = mod._forward(x, w, b, None, None, mod.ACTIVATIONS[act], True)
+    want = x.double() + b.double()
+    chunk = e.repeat_interleave(32, 1)[:, :N].double()
+    got = z.double() * torch.exp2(chunk - 141)
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got)) and torch.equal(torch.isnan(want), torch.isnan(got))
+    tol = (2.0 ** -11 + 2.0 ** -23) * want.abs() + 2.0 ** -25 * torch.exp2(chunk - 141)
+    assert bool(((got - want).abs() <= tol)[fine].all())
+    assert bool((torch.exp2(chunk - 141) <= torch.maximum(want.abs()[fine].max(), want.new_tensor(2.0 ** -100)))[fine].all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ACTS)
 def test_saturated_activations(act, dtype):
