@@ -433,15 +433,18 @@ static cudaError_t balance_launch(const b200_balance_args& a, cudaStream_t st) {
 
 // Lanes per token: 16 experts a lane, so that a warp has several tokens in work and what is done once per token (shuffles,
 // addresses, counts) is shared; with 8 a lane the kernels took half as many instructions again.
+// Rows that do not start on 16 bytes have fewer forms.
 template <bool BACK, typename T, int V>
 static cudaError_t balance_lanes(const b200_balance_args& a, cudaStream_t st) {
   constexpr int P = 16 / V;
-  if (a.E <= 8 && V > 1) return balance_launch<BACK, T, 1, V, 8 / V>(a, st);
+  if constexpr (V > 1) {
+    if (a.E <= 8) return balance_launch<BACK, T, 1, V, 8 / V>(a, st);
+    if (a.E > 16 && a.E <= 32) return balance_launch<BACK, T, 2, V, P>(a, st);
+    if (a.E > 32 && a.E <= 64) return balance_launch<BACK, T, 4, V, P>(a, st);
+    if (a.E > 128 && a.E <= 256) return balance_launch<BACK, T, 16, V, P>(a, st);
+  }
   if (a.E <= 16) return balance_launch<BACK, T, 1, V, P>(a, st);
-  if (a.E <= 32) return balance_launch<BACK, T, 2, V, P>(a, st);
-  if (a.E <= 64) return balance_launch<BACK, T, 4, V, P>(a, st);
   if (a.E <= 128) return balance_launch<BACK, T, 8, V, P>(a, st);
-  if (a.E <= 256) return balance_launch<BACK, T, 16, V, P>(a, st);
   if (a.E <= 512) return balance_launch<BACK, T, 32, V, P>(a, st);
   return balance_launch<BACK, T, 32, V, 2 * P>(a, st);
 }

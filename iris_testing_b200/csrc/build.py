@@ -3,7 +3,7 @@
 Every ``.cu`` / ``.cpp`` file in this directory is compiled for sm_100a with
 nvcc and linked into one shared object that Python loads through ``ctypes``.
 The kernels take raw device pointers and a stream handle, so no PyTorch header
-is needed and a full rebuild takes seconds.  A stamp file next to the library
+is needed and a full rebuild takes about a minute.  A stamp file next to the library
 holds a hash of the sources; ``build()`` is a no-op while it matches.
 
 Usage: ``python -m iris_testing_b200.csrc.build [--force] [--verbose]``
