@@ -218,7 +218,13 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_fo
   if constexpr (S > 0) async_wait<0>();
 }
 
-template <typename T, int VEC, int VPT, int MAXT>
+// FORM says which of two conditions hold, a next norm and a gate of the rows' own shape, both of which stand around every
+// pack: known beforehand they cost neither registers nor branches.  Found out at run time (NORM_ANY) the kernel took 88 us
+// for 8192 x 4096 with a next norm, and 79 for 5003 x 6144 without one; as forms of their own 74 and 61.  Rows that do not
+// lie on 16 bytes, and those of more than 8192 columns, keep the one kernel for all.
+enum NormForm : int { NORM_NEXT = 1, NORM_FULL_GATE = 2, NORM_ANY = 4 };
+
+template <typename T, int VEC, int VPT, int MAXT, int FORM>
 __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_backward_kernel(const b200_norm_args a) {
   extern __shared__ uint4 slots[];
   __shared__ __align__(16) float sums[2][2][32];
@@ -229,7 +235,8 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_ba
   const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
   const int threads = blockDim.x, stride = (WARP_ROW ? 32 : threads) * VEC;
   const float inv_h = 1.f / static_cast<float>(a.H);
-  const bool next = a.dn != nullptr;
+  const bool next = FORM == NORM_ANY ? a.dn != nullptr : (FORM & NORM_NEXT) != 0;
+  const bool full_gate = FORM == NORM_ANY ? a.gate_kind == 3 : (FORM & NORM_FULL_GATE) != 0;
   // [w times gate, w2][VPT][VQ][threads], then [stage][y, dh, res, dn][VPT][threads]: a thread's own, all of them
   float4* factors = reinterpret_cast<float4*>(slots) + threadIdx.x;
   uint4* mine = slots + (S > 0 ? 2 * VPT * VQ * threads : 0) + threadIdx.x;
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_ba
     const float r1 = n1, r2 = n2, gate_row = ng;
     numbers(row + a.parts);
     auto times_full_gate = [&](int c, float (&x)[VEC]) {
-      if (a.gate_kind != 3) return;
+      if (!full_gate) return;
       float g[VEC];
       load_pack<T, VEC>(static_cast<const T*>(a.gate) + row * a.ld_gate + c, g);
       v_mul<VEC>(x, x, g);
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_ba
       // A takes in a gate that changes from row to row; gh becomes q but for the row's gate
       float g[VEC];
       v_mul<VEC>(g, d, gate_row);
-      if (a.gate_kind == 3) {
+      if (full_gate) {
         float p[VEC];
         v_mul<VEC>(p, d, f);
         v_mul<VEC>(p, p, yh[i]);
@@ -462,6 +469,7 @@ static int norm_parts(int T, int threads, size_t smem, int sms) {
 
 template <bool BACK, typename T, int VEC, int VPT, int MAXT>
 static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
+  using Kernel = void (*)(const b200_norm_args);
   const int threads = norm_row_threads<MAXT>(a.H, VEC, VPT);
   const int block = MAXT == 32 ? NORM_WARP_ROWS * 32 : threads;
   const int tensors = BACK ? (a.dn != nullptr ? 4 : 2) : (a.res != nullptr ? 2 : 1);
@@ -469,10 +477,22 @@ static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
   const size_t smem = (static_cast<size_t>(S) * tensors * VPT * 16 + (BACK && S > 0 ? 2 * VPT * VEC * 4 : 0)) * block;   // at most 200 KB
   a.parts = norm_parts<MAXT>(a.T, threads, smem, sms);
   const dim3 grid(MAXT == 32 ? a.parts / NORM_WARP_ROWS : a.parts);
-  auto kern = BACK ? norm_backward_kernel<T, VEC, VPT, MAXT> : norm_forward_kernel<T, VEC, VPT, MAXT>;
-  static std::atomic<unsigned long long> allowed{0};
+  Kernel kern;
+  int form = 0;
+  if constexpr (!BACK) {
+    kern = norm_forward_kernel<T, VEC, VPT, MAXT>;
+  } else if constexpr (S == 0) {
+    kern = norm_backward_kernel<T, VEC, VPT, MAXT, NORM_ANY>;
+  } else {
+    form = (a.dn != nullptr ? NORM_NEXT : 0) | (a.gate_kind == 3 ? NORM_FULL_GATE : 0);
+    kern = form == 0 ? norm_backward_kernel<T, VEC, VPT, MAXT, 0>
+         : form == NORM_NEXT ? norm_backward_kernel<T, VEC, VPT, MAXT, NORM_NEXT>
+         : form == NORM_FULL_GATE ? norm_backward_kernel<T, VEC, VPT, MAXT, NORM_FULL_GATE>
+                                  : norm_backward_kernel<T, VEC, VPT, MAXT, NORM_NEXT | NORM_FULL_GATE>;
+  }
+  static std::atomic<unsigned long long> allowed[4];
   if (S > 0) {
-    const cudaError_t e = allow_shared_memory(kern, NORM_SLOT_BYTES, allowed);
+    const cudaError_t e = allow_shared_memory(kern, NORM_SLOT_BYTES, allowed[form]);
     if (e != cudaSuccess) return e;
   }
   b200_count_launches(1);
