@@ -60,9 +60,12 @@ constexpr int NORM_WARP_ROWS = 4;      // rows of a block where a warp has a row
 constexpr int NORM_ELEMS = 16;         // elements of a row per thread (8 where that is enough)
 
 // Threads of a block and blocks of an SM of a variant: MAXT is the most threads that share a row (32: a warp).  512
-// threads an SM leave 128 registers each; where 1024 threads share a row (more than 8192 columns) it is 64.
-template <int MAXT>
-constexpr int NORM_BLOCKS = MAXT == 32 ? 4 : MAXT == 256 ? 2 : 1;
+// threads an SM leave 128 registers each; where 1024 threads share a row (more than 8192 columns) it is 64.  The forward
+// kernel of 16-bit rows above 4096 and up to 6144 columns needs 78 and so has two blocks of 384 threads on an SM instead of
+// one: 8192 rows of 5120 columns 52 -> 40 us, with a residual 58 -> 48, with a next norm 75 -> 62; of 6144 columns
+// 52 -> 44, 59 -> 56, 77 -> 77.  For fp32 rows the two are even (68 -> 62, 87 -> 93, 122 -> 118), and one block stays.
+template <bool BACK, int MAXT>
+constexpr int NORM_BLOCKS = MAXT == 32 ? 4 : MAXT == 256 || (MAXT == 384 && !BACK) ? 2 : 1;
 template <int MAXT>
 constexpr int NORM_THREADS = MAXT == 32 ? NORM_WARP_ROWS * 32 : MAXT;
 // Rows on their way ahead of the one in work: up to three, by the slots that fit beside each other on an SM (two tensors
@@ -72,7 +75,7 @@ constexpr int NORM_SLOT_BYTES = 200 * 1024;
 template <bool BACK, int VEC, int VPT, int MAXT>
 constexpr int NORM_VECTOR_BYTES = BACK && VEC > 1 && MAXT != 1024 ? 2 * VPT * VEC * 4 * NORM_THREADS<MAXT> : 0;
 template <bool BACK, int VEC, int VPT, int MAXT>
-constexpr int NORM_FIT = (NORM_SLOT_BYTES / NORM_BLOCKS<MAXT> - NORM_VECTOR_BYTES<BACK, VEC, VPT, MAXT>) / ((BACK ? 4 : 2) * VPT * 16 * NORM_THREADS<MAXT>);
+constexpr int NORM_FIT = (NORM_SLOT_BYTES / NORM_BLOCKS<BACK, MAXT> - NORM_VECTOR_BYTES<BACK, VEC, VPT, MAXT>) / ((BACK ? 4 : 2) * VPT * 16 * NORM_THREADS<MAXT>);
 template <bool BACK, int VEC, int VPT, int MAXT>
 constexpr int NORM_STAGES = VEC == 1 || MAXT == 1024 ? 0 : NORM_FIT<BACK, VEC, VPT, MAXT> < 3 ? NORM_FIT<BACK, VEC, VPT, MAXT> : 3;
 
@@ -116,7 +119,7 @@ __device__ __forceinline__ float row_factor(const b200_norm_args& a, int row) {
 }
 
 template <typename T, int VEC, int VPT, int MAXT>
-__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_forward_kernel(const b200_norm_args a) {
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<false, MAXT>) norm_forward_kernel(const b200_norm_args a) {
   extern __shared__ uint4 slots[];
   __shared__ __align__(16) float sums[2][2][32];       // two sets: a row's sums while a slow warp still reads the row before's
   constexpr bool WARP_ROW = MAXT == 32;
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_fo
 enum NormForm : int { NORM_NEXT = 1, NORM_FULL_GATE = 2, NORM_ANY = 4 };
 
 template <typename T, int VEC, int VPT, int MAXT, int FORM>
-__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<MAXT>) norm_backward_kernel(const b200_norm_args a) {
+__global__ void __launch_bounds__(NORM_THREADS<MAXT>, NORM_BLOCKS<true, MAXT>) norm_backward_kernel(const b200_norm_args a) {
   extern __shared__ uint4 slots[];
   __shared__ __align__(16) float sums[2][2][32];
   constexpr bool WARP_ROW = MAXT == 32;
@@ -457,10 +460,10 @@ static int norm_row_threads(int H, int vec, int vpt) {
 
 // Rows (of warps, or of blocks) in work at once: the blocks that the registers of the variant and the slots leave room
 // for on every SM, and no more rows than there are.
-template <int MAXT>
+template <bool BACK, int MAXT>
 static int norm_parts(int T, int threads, size_t smem, int sms) {
   const int rows = MAXT == 32 ? NORM_WARP_ROWS : 1;
-  int per_sm = MAXT == 32 ? NORM_BLOCKS<32> : MAXT * NORM_BLOCKS<MAXT> / threads;
+  int per_sm = MAXT == 32 ? NORM_BLOCKS<BACK, 32> : MAXT * NORM_BLOCKS<BACK, MAXT> / threads;
   const int fit = static_cast<int>((224u * 1024u) / (smem + 2048));      // beside 1 KB of the system's and the sums
   if (fit < per_sm) per_sm = fit > 0 ? fit : 1;
   const int blocks = (T + rows - 1) / rows;
@@ -475,7 +478,7 @@ static cudaError_t norm_launch(b200_norm_args a, int sms, cudaStream_t st) {
   const int tensors = BACK ? (a.dn != nullptr ? 4 : 2) : (a.res != nullptr ? 2 : 1);
   constexpr int S = NORM_STAGES<BACK, VEC, VPT, MAXT>;
   const size_t smem = (static_cast<size_t>(S) * tensors * VPT * 16 + (BACK && S > 0 ? 2 * VPT * VEC * 4 : 0)) * block;   // at most 200 KB
-  a.parts = norm_parts<MAXT>(a.T, threads, smem, sms);
+  a.parts = norm_parts<BACK, MAXT>(a.T, threads, smem, sms);
   const dim3 grid(MAXT == 32 ? a.parts / NORM_WARP_ROWS : a.parts);
   Kernel kern;
   int form = 0;
@@ -515,6 +518,8 @@ static auto norm_variant(int H, bool aligned, F&& f) {
   if (H <= 256) return f.template operator()<V, 8 / V, 32>();
   if (H <= 32 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 32>();
   if (H <= 256 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 256>();
+  if constexpr (V == 8)
+    if (H <= 384 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 384>();
   if (H <= 512 * NORM_ELEMS) return f.template operator()<V, NORM_ELEMS / V, 512>();
   return f.template operator()<V, NORM_ELEMS / V, 1024>();
 }
@@ -537,7 +542,7 @@ static int norm_dispatch(bool back, const b200_norm_args& a, int sms, cudaStream
 struct NormPartsOf {
   int T, H, sms;
   template <int VEC, int VPT, int MAXT>
-  int operator()() const { return norm_parts<MAXT>(T, norm_row_threads<MAXT>(H, VEC, VPT), 0, sms); }
+  int operator()() const { return norm_parts<true, MAXT>(T, norm_row_threads<MAXT>(H, VEC, VPT), 0, sms); }
 };
 
 template <bool BACK>
