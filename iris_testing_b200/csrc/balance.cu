@@ -54,6 +54,7 @@ namespace b200 {
 
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_E = 1024;
+constexpr int BAL_MOST = 0x7fffffff - 0xfffff;      // tokens, and blocks of 32 experts of all sequences: their numbers have 32 bits
 // Blocks of an SM: as many runs as these make no second, half empty round.
 constexpr int BAL_FORWARD_BLOCKS = 4, BAL_BACKWARD_BLOCKS = 3;
 
@@ -458,8 +459,9 @@ static cudaError_t balance_dispatch(const b200_balance_args& a, cudaStream_t st)
 
 template <bool BACK>
 static int balance_run(const b200_balance_args* a, void* stream) {
-  if (a == nullptr || a->T < 1 || a->E < 1 || a->E > BAL_MAX_E || a->k < 1 || a->S < 1 || a->runs < 1 || a->run_tokens < 1 ||
-      static_cast<long long>(a->runs) * a->run_tokens < a->T || static_cast<long long>(a->runs - 1) * a->run_tokens >= a->T)
+  if (a == nullptr || a->T < 1 || a->T > BAL_MOST || a->E < 1 || a->E > BAL_MAX_E || a->k < 1 || a->S < 1 || a->runs < 1 || a->run_tokens < 1 ||
+      static_cast<long long>(a->runs) * a->run_tokens < a->T || static_cast<long long>(a->runs - 1) * a->run_tokens >= a->T ||
+      static_cast<long long>(a->S) * ((a->E + 31) / 32) > BAL_MOST)
     return -10;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a->elem) {

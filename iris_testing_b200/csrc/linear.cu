@@ -84,6 +84,7 @@ constexpr int LBN = 256;                 // columns of a tile
 constexpr int LBK = 64;                  // contracted elements per stage
 constexpr int LIN_THREADS = 256;
 constexpr int LIN_MENDERS = 2;           // warps 6 and 7
+constexpr int LIN_MAX_ROWS = 0x7fffffff - 1023;      // a last tile that is partly empty still has row numbers of 32 bits
 constexpr int LIN_A_BYTES = LBM * LBK * 2;
 constexpr int LIN_MN_BOX = 64 * LBK * 2; // bytes of one MN-major box
 constexpr int LIN_BOX = 32 * 128;        // a warp's staging box: 32 rows x 64 columns, 16-byte chunks XOR-swizzled by row
@@ -1238,7 +1239,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   b200_linear_args la = *args;
   if (la.N % 8 != 0 || la.K % 8 != 0 || (la.elem != ELEM_BF16 && la.elem != ELEM_F16)) return -11;
   if (la.mode < LIN_FORWARD || la.mode > LIN_DW) return -15;
-  if ((la.group_rows == nullptr && la.G != 1) || static_cast<long long>(la.G) * la.N > 0x7fffffffll) return -12;
+  if ((la.group_rows == nullptr && la.G != 1) || la.M > LIN_MAX_ROWS || static_cast<long long>(la.G) * la.N > LIN_MAX_ROWS) return -12;
   const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
   if (gated && la.N % 256 != 0) return -13;
   if ((la.z != nullptr) != (la.zexp != nullptr)) return -17;

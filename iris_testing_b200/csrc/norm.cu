@@ -56,6 +56,7 @@ typedef struct b200_norm_args {
 namespace b200 {
 
 constexpr int NORM_MAX_H = 16384;
+constexpr int NORM_MAX_ROWS = 1 << 30;  // rows ahead of the last one still have numbers of 32 bits
 constexpr int NORM_WARP_ROWS = 4;      // rows of a block where a warp has a row
 constexpr int NORM_ELEMS = 16;         // elements of a row per thread (8 where that is enough)
 
@@ -547,7 +548,7 @@ struct NormPartsOf {
 
 template <bool BACK>
 static int norm_run(const b200_norm_args* a, int sms, void* stream) {
-  if (a == nullptr || sms < 1 || a->T < 1 || a->H < 1 || a->H > NORM_MAX_H || a->y == nullptr || a->gate_kind < 0 || a->gate_kind > 3) return -10;
+  if (a == nullptr || sms < 1 || a->T < 1 || a->T > NORM_MAX_ROWS || a->H < 1 || a->H > NORM_MAX_H || a->y == nullptr || a->gate_kind < 0 || a->gate_kind > 3) return -10;
   if ((a->gate_kind != 0 && (a->gate == nullptr || a->res == nullptr)) || (a->w2 != nullptr && a->res == nullptr)) return -11;
   if (!BACK && (a->h == nullptr || (a->w2 != nullptr && a->n == nullptr))) return -12;
   if (BACK && ((a->norm && a->r1 == nullptr) || (a->dn != nullptr && (a->r2 == nullptr || a->w2 == nullptr)))) return -13;

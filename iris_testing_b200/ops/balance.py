@@ -16,6 +16,7 @@ from ._common import (ELEM, Entry, declare, launch_status, on_device, require, r
 from .expert import sm_count
 
 MAX_BALANCE_EXPERTS = 1024
+MAX_TOKENS = 2 ** 31 - 2 ** 20      # also of the blocks of 32 experts of all sequences
 
 
 class BalanceArgs(C.Structure):
@@ -145,6 +146,8 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
         raise ValueError(f"logits must be float32, bfloat16 or float16 (got {logits.dtype})")
     if E > MAX_BALANCE_EXPERTS:
         raise ValueError(f"at most {MAX_BALANCE_EXPERTS} experts (got {E})")
+    if T > MAX_TOKENS or (seq_rows is not None and seq_rows.numel() * -(-E // 32) > MAX_TOKENS):
+        raise ValueError(f"at most {MAX_TOKENS} tokens, and blocks of 32 experts of all sequences")
     require_device(logits.device, topk_idx=topk_idx, seq_rows=seq_rows, token_mask=token_mask)
     logits, idx = rows_view(logits), topk_idx.contiguous()
     if seq_rows is not None:

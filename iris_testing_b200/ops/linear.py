@@ -19,6 +19,7 @@ from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
 _FORWARD, _DX, _DW = 0, 1, 2
+MAX_ROWS = 2 ** 31 - 1024        # a last tile that is partly empty still has row numbers of 32 bits
 
 
 def _run_rows(M: int, n_out: int) -> int:
@@ -223,7 +224,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     require(w_kmajor.dtype == dt and (bias is None or bias.dtype == dt) and (residual is None or residual.dtype == dt),
             "w_kmajor, bias and residual must have x's dtype")
     require(K % 8 == 0 and N % 8 == 0, "K and N must be multiples of 8")
-    require(x.numel() // K < 2 ** 31 and G * N < 2 ** 31, "too many rows")
+    if x.numel() // K > MAX_ROWS or G * N > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows of x, and of the weights of all groups")
     require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)
     flat = len(shape) == 2                   # no views, which autograd would have to pass through
     x2 = _plain(x if flat else x.reshape(-1, K))

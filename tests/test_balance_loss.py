@@ -241,6 +241,7 @@ def test_refusals_on_the_gpu():
     for bad in (lambda: ops.balance_loss(lg.double(), idx),
                 lambda: ops.balance_loss(lg, idx.cpu()),
                 lambda: ops.balance_loss(lg, idx, seq_rows=torch.tensor([6], dtype=torch.int32)),
+                lambda: ops.balance_loss(lg[:1].expand(2 ** 31 - 1000, 4), idx[:1].expand(2 ** 31 - 1000, 2)),
                 lambda: ops.balance_loss(torch.randn(2, 1025, device="cuda"), idx[:2])):
         with pytest.raises(ValueError):
             bad()

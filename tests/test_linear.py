@@ -371,6 +371,7 @@ def test_refusals_on_the_gpu():
                 lambda: ops.linear(x[:, :12], w[:, :12]),
                 lambda: ops.linear(x, w[:252]),
                 lambda: ops.linear(x, w, torch.ones(256, device="cuda")),
+                lambda: ops.linear(x[:1].expand(2 ** 31 - 1000, 16), w),       # a view of one row
                 lambda: ops.linear(x, torch.ones(129, 8, 16, device="cuda", dtype=torch.bfloat16),
                                    group_rows=torch.zeros(129, dtype=torch.int32, device="cuda"))):
         with pytest.raises(ValueError):

@@ -46,12 +46,18 @@ def test_entries_refuse_bad_arguments_without_a_gpu():
     assert lib.b200_norm_forward(C.byref(n), 148, None) < 0
     n.H, n.gate_kind = 64, 1                       # a gate without a residual
     assert lib.b200_norm_forward(C.byref(n), 148, None) < 0
+    n.H, n.gate_kind, n.T = 64, 0, (1 << 30) + 1
+    assert lib.b200_norm_forward(C.byref(n), 148, None) < 0
     b = BalanceArgs()
     b.T, b.E, b.k, b.S, b.runs, b.run_tokens = 10, 8, 2, 1, 2, 4       # runs that do not cover the tokens
     assert lib.b200_balance_forward(C.byref(b), None) < 0
-    b.run_tokens, b.E = 5, 1025
+    b.T, b.runs, b.run_tokens = 2 ** 31 - 1000, 1, 2 ** 31 - 1000
     assert lib.b200_balance_forward(C.byref(b), None) < 0
-    for field, value in (("N", 60), ("K", 4), ("G", 129), ("G", 2), ("M", 0), ("n_out", 128), ("elem", 0), ("mode", 3)):
+    b.T, b.runs, b.run_tokens, b.S = 10, 2, 5, 2 ** 31 - 1000
+    assert lib.b200_balance_forward(C.byref(b), None) < 0
+    b.S, b.E = 1, 1025
+    assert lib.b200_balance_forward(C.byref(b), None) < 0
+    for field, value in (("N", 60), ("K", 4), ("G", 129), ("G", 2), ("M", 0), ("M", 2 ** 31 - 1000), ("n_out", 128), ("elem", 0), ("mode", 3)):
         la = _split_args(linear)
         setattr(la, field, value)
         assert lib.b200_linear(C.byref(la), 148, None) < 0, field
