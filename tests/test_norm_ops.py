@@ -184,6 +184,14 @@ def test_norms_at_the_ends_of_the_range(T, H, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["full", "full next", "row", "channel next w32"])
+@pytest.mark.parametrize("T,H", [(1301, 4104), (1000, 6144), (500, 8184), (400, 8200), (700, 4099)])
+def test_several_wide_rows_per_block(T, H, kind, dtype):
+    check(make(T, H, dtype, kind, "cuda"), 0.5, kind)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["pre", "full next", "row next"])
 @pytest.mark.parametrize("how", ["strided", "shifted", "expanded", "3d"])
 def test_layouts(how, kind):
