@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nv
 
@@ -47,6 +48,16 @@ def require_device(device: torch.device, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise ValueError(f"{name} must be on {device} (got {t.device})")
+
+
+def refuse_tangents(**tensors) -> None:
+    """Refuses tensors that carry a forward-mode tangent: a kernel works on the values alone, and a result without a tangent
+    would read as a derivative of zero.  Outside of a dual level, which is where nearly all calls are, nothing is looked at."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} carries a tangent: forward-mode derivatives are only there for CPU tensors")
 
 
 class _Here:

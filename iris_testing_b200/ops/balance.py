@@ -11,8 +11,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import cpu_ref
-from ._common import (ELEM, Entry, declare, launch_status, on_device, require, require_device, rows_view, stream_ptr,
-                      use_native)
+from ._common import (ELEM, Entry, declare, launch_status, on_device, refuse_tangents, require, require_device, rows_view,
+                      stream_ptr, use_native)
 from .expert import sm_count
 
 MAX_BALANCE_EXPERTS = 1024
@@ -96,6 +96,7 @@ class _Balance(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss, _):
+        refuse_tangents(dloss=dloss)
         logits, seq_rows, mask, keep = ctx.saved_tensors
         if dloss is None:
             return (None,) * 6
@@ -132,7 +133,8 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
     A token also takes no part where its logits hold a NaN or +infinity, or nothing above their type's lowest value (all
     experts masked).  Such tokens get a zero gradient, sequences without any token are left out of the mean, and
     without any token at all the loss is zero.  ``counts`` is [E], or [S, E] with ``seq_rows``; it may be changed by the
-    caller.  The same inputs give the same bits.  CPU tensors take plain PyTorch."""
+    caller.  The same inputs give the same bits.  Derivatives are reverse mode, of first order.  CPU tensors take plain
+    PyTorch."""
     require(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be [T, E]")
     T, E = logits.shape
     require(topk_idx.dim() == 2 and topk_idx.shape[0] == T and topk_idx.shape[1] >= 1, "topk_idx must be [T, k]")
@@ -149,6 +151,7 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
     if T > MAX_TOKENS or (seq_rows is not None and seq_rows.numel() * -(-E // 32) > MAX_TOKENS):
         raise ValueError(f"at most {MAX_TOKENS} tokens, and blocks of 32 experts of all sequences")
     require_device(logits.device, topk_idx=topk_idx, seq_rows=seq_rows, token_mask=token_mask)
+    refuse_tangents(logits=logits)
     logits, idx = rows_view(logits), topk_idx.contiguous()
     if seq_rows is not None:
         seq_rows = seq_rows.contiguous()

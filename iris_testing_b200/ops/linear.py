@@ -14,7 +14,7 @@ import torch
 
 from .. import _native as nv
 from . import cpu_ref
-from ._common import ELEM, Entry, declare, launch_status, on_device, require, require_device, stream_ptr, use_native
+from ._common import ELEM, Entry, declare, launch_status, on_device, refuse_tangents, require, require_device, stream_ptr, use_native
 from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
@@ -174,6 +174,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_tangents(dy=dy)
         x, w, z, exponents, group_rows = ctx.saved_tensors
         has_bias, has_res, act = ctx.how
         return (*_backward(x, w, (z, exponents), has_bias, has_res, group_rows, act, ctx.needs_input_grad[:4], _plain(dy)), None, None)
@@ -194,8 +195,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
 
     All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
     the pre-activation is kept to 11 bits and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
-    timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.  CPU tensors take
-    plain PyTorch."""
+    timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.
+    Derivatives are reverse mode, of first order.  CPU tensors take plain PyTorch."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)} (got {activation!r})")
     grouped = group_rows is not None
@@ -227,6 +228,7 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     if x.numel() // K > MAX_ROWS or G * N > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows of x, and of the weights of all groups")
     require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)
+    refuse_tangents(x=x, w_kmajor=w_kmajor, bias=bias, residual=residual)
     flat = len(shape) == 2                   # no views, which autograd would have to pass through
     x2 = _plain(x if flat else x.reshape(-1, K))
     r2 = residual if residual is None or flat else residual.reshape(-1, n_out)

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import cpu_ref
-from ._common import ELEM, Entry, declare, on_device, require, require_device, rows_view, stream_ptr, use_native
+from ._common import ELEM, Entry, declare, on_device, refuse_tangents, require, require_device, rows_view, stream_ptr, use_native
 from .expert import sm_count
 
 GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
@@ -189,10 +189,12 @@ class _Norm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dn=None):
+        refuse_tangents(dh=dh, dn=dn)
         return (*_backward(ctx.saved_tensors, *ctx.how, ctx.needs_input_grad[:5], dh, dn), None, None, None, None)
 
 
 def _apply(y, residual, weight, gate, next_weight, kind, norm, scale, eps):
+    refuse_tangents(y=y, residual=residual, weight=weight, gate=gate, next_weight=next_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, residual, weight, gate, next_weight)):
         return _Norm.apply(y, residual, weight, gate, next_weight, kind, norm, scale, eps)
     h, n, _ = _forward(y, residual, weight, gate, kind, norm, scale, next_weight, eps, False)
@@ -205,7 +207,8 @@ def pre_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: flo
     x       [..., H] float32, bfloat16 or float16, H <= 16384; rows may be strided
     weight  [H] in x's dtype or float32, or None
 
-    Statistics and products are fp32, rounded once.  CPU tensors take plain PyTorch."""
+    Statistics and products are fp32, rounded once.  Derivatives are reverse mode, of first order.  CPU tensors take plain
+    PyTorch."""
     _check(x, None, weight, None, None)
     if not use_native(x):
         return cpu_ref.rms_norm_ref(x, weight, eps).to(x.dtype)
@@ -224,7 +227,7 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Te
     next_weight  [H]: weight of the norm in front of the next block, in y's dtype or float32
 
     n is the norm of h before h is rounded.  Gradients of weight, gate and next_weight are summed in fp32 in a fixed
-    order: the same inputs give the same bits.  CPU tensors take plain PyTorch."""
+    order: the same inputs give the same bits.  Derivatives are reverse mode, of first order.  CPU tensors take plain PyTorch."""
     require(norm or weight is None, "weight belongs to the norm of y: norm=False takes none")
     require(residual is not None, "post_norm needs the residual (pre_norm is the norm alone)")
     kind = _check(y, residual, weight, gate, next_weight)
