@@ -190,8 +190,9 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     bias        [N] or [G, N];  residual [..., n_out]: what is added after the activation
     activation  None, "relu", "silu", "gelu" (tanh form), or "silu_gate": every 256 rows of w hold 128 gate rows and
                 then 128 up rows, the result is silu(gate) * up and n_out = N / 2
-    group_rows  int32 [G] on x's device: rows of each group, none allowed.  Rows of x behind the last group are not read;
-                the result and the gradients of x and residual are zero there.
+    group_rows  int32 [G] on x's device: rows of each group, none allowed (of copies packed by expert: ``make_plan``'s
+                counts; those of a balance loss leave some out).  Rows of x behind the last group are not read; the result
+                and the gradients of x and residual are zero there.
 
     All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
     the pre-activation is kept to 11 bits and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
