@@ -20,8 +20,11 @@
 // 603 for 1024 rows, which need none).
 //
 // The pre-activations z are kept for the backward pass as fp16 under a power of two that 32 columns of a row share, kept in a
-// byte: 11 bits of precision in fp32's range.  (Kept as bf16, they put dX and dW of a gated bf16 product 3.0e-3 off
-// instead of 2.4e-3, relative; 1.7e-3 is what rounding the result alone costs.)
+// byte: off by 2^-11 |z|, and by 2^-30 in absolute terms.  fp16 spans too little for 32 columns that hold both a value of
+// 1024 or more and one 2^31 times smaller than it: those are kept as bf16, off by 2^-8 |z| whatever the size (beside
+// 1e12, a 1 under a shared power of two would be kept as nothing, and its slope and its products with it).  (Kept as bf16
+// throughout, dX and dW of a gated bf16 product are 3.0e-3 off instead of 2.4e-3, relative; 1.7e-3 is what rounding the result
+// alone costs.)
 // dz is rounded to the element type, since the tensor cores multiply 16-bit values: at most half a step of each value, which
 // averages out over the contracted dimension.
 #include <cuda.h>
@@ -44,7 +47,7 @@ typedef struct b200_linear_args {
   const void* a;            // forward: x [M, K]; dX: dz [M, N]; dW: dz [M, N]
   const void* b;            // forward, dX: W [G, N, K]; dW: x [M, K]
   void* out;                // y [M, n_out]; dx [M, K]; dW [G, N, K]
-  void* z;                  // forward: fp16 [M, N] or null
+  void* z;                  // forward: [M, N] of 16 bits or null: fp16 under the powers of two of zexp, or bf16
   unsigned char* zexp;      // with z: [M][ceil(N / 256) * 8], exponents of 32 columns each
   const void* bias;         // [G, N] or null
   const void* res;          // [M, n_out] or null
@@ -62,7 +65,7 @@ typedef struct b200_linear_args {
 
 typedef struct b200_act_grad_args {
   const void* dy;           // [M, n_out]
-  const void* z;            // fp16 [M, N] or null (no activation)
+  const void* z;            // [M, N] as the forward product left it, or null (no activation)
   const unsigned char* zexp;   // as the forward product left it
   void* dz;                 // [M, N] or null (no activation: dz is dy)
   void* dres;               // [M, n_out] or null: dy of the groups' rows, zero behind them
@@ -145,10 +148,15 @@ __device__ __forceinline__ float act_slope(float v, int act) {
 }
 
 // z in fp16 under a shared power of two: E is the largest finite magnitude's exponent (biased, 15 at least), the
-// values are scaled into [0, 2^15], where fp16 has 11 bits down to 2^-14.  Infinities and NaN stay what they are.
+// values are scaled into [0, 2^15], where fp16 has 11 bits down to 2^-14, 8 down to 2^-17 and an absolute error of 2^-25.
+// Infinities and NaN stay what they are; so near to fp32's largest value that rounding reaches 2^128, z becomes infinite.
+// Scales of 2^-5 and below (E >= 137: a value of 1024) leave an absolute error that ordinary values may feel: there, where the
+// smallest that is not zero lies below the 8 bits, the values are bf16, and the byte is Z_BF16.
+constexpr int Z_BF16 = 255;
 __device__ __forceinline__ int shared_exponent(uint32_t largest_finite_bits) { return max(15, static_cast<int>(largest_finite_bits >> 23)); }
 __device__ __forceinline__ float z_scale(int E) { return __uint_as_float(static_cast<uint32_t>(268 - E) << 23); }      // 2^(141 - E)
 __device__ __forceinline__ float z_unscale(int E) { return __uint_as_float(static_cast<uint32_t>(E - 14) << 23); }    // 2^(E - 141)
+__device__ __forceinline__ bool z_spans_much(int E, float smallest) { return E >= 137 && smallest * z_scale(E) < 0x1p-17f; }
 __device__ __forceinline__ long long zexp_pitch(int N) { return (N + 255) / 256 * 8; }
 
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
@@ -533,16 +541,27 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
                     if (col + (i & ~7) < la.N && f <= 3.402823466e38f) m = fmaxf(m, f);
                   }
                 }
-                const int E = shared_exponent(__float_as_uint(m));
-                const float s = z_scale(E);
+                int E = shared_exponent(__float_as_uint(m));
+                if (E >= 137) {                        // rare
+                  float least = m;
+                  for (int i = 0; i < 32; ++i) {
+                    const float f = fabsf(__uint_as_float(x[i]));
+                    if (col + (i & ~7) < la.N && f > 0.f) least = fminf(least, f);
+                  }
+                  if (z_spans_much(E, least)) E = Z_BF16;
+                }
                 exponents |= static_cast<unsigned long long>(E) << (8 * chunk);
+                auto fill = [&](float s, bool as_bf16) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
-                      make_uint4(pack_16(__uint_as_float(x[8 * i]) * s, __uint_as_float(x[8 * i + 1]) * s, false),
-                                 pack_16(__uint_as_float(x[8 * i + 2]) * s, __uint_as_float(x[8 * i + 3]) * s, false),
-                                 pack_16(__uint_as_float(x[8 * i + 4]) * s, __uint_as_float(x[8 * i + 5]) * s, false),
-                                 pack_16(__uint_as_float(x[8 * i + 6]) * s, __uint_as_float(x[8 * i + 7]) * s, false));
+                  for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
+                        make_uint4(pack_16(__uint_as_float(x[8 * i]) * s, __uint_as_float(x[8 * i + 1]) * s, as_bf16),
+                                   pack_16(__uint_as_float(x[8 * i + 2]) * s, __uint_as_float(x[8 * i + 3]) * s, as_bf16),
+                                   pack_16(__uint_as_float(x[8 * i + 4]) * s, __uint_as_float(x[8 * i + 5]) * s, as_bf16),
+                                   pack_16(__uint_as_float(x[8 * i + 6]) * s, __uint_as_float(x[8 * i + 7]) * s, as_bf16));
+                };
+                if (E != Z_BF16) fill(z_scale(E), false);
+                else fill(1.f, true);
               };
               put(v, zbox, zcol, p * 2 + h);
               if constexpr (GATED) put(reinterpret_cast<uint32_t(&)[32]>(u), ubox, zcol + LBN / 2, 4 + p * 2 + h);
@@ -643,6 +662,16 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   }
 }
 
+// Eight values of z as they were kept.
+__device__ __forceinline__ void kept_z(const Pack<__half, 8>& k, int e, float (&v)[8]) {
+  if (e == Z_BF16) {
+    unpack<__nv_bfloat16, 8>(*reinterpret_cast<const Pack<__nv_bfloat16, 8>*>(&k), v);
+  } else {
+    unpack<__half, 8>(k, v);
+    v_mul<8>(v, v, z_unscale(e));
+  }
+}
+
 // dz = act'(z) dy and the column sums of dz over each group.  A thread takes eight columns of the output down a run of
 // rows, the next row under way while it works on one; the sums of a (run, group) go to record run + group (both only ever
 // advance), added up in order by the next kernel.  Bound by memory traffic with SUMS off; 64 registers, so that an SM holds
@@ -693,19 +722,17 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
     for (long long r = pos; r < end; ++r) {
       const P cd = kd;
       const Z cz = kz, cu = ku;
-      const float sz = z_unscale(ez), su = z_unscale(eu);
+      const int cez = ez, ceu = eu;
       if (r + 1 < end) load(r + 1);
       if (a.dres != nullptr) *reinterpret_cast<P*>(static_cast<T*>(a.dres) + r * a.n_out + oc) = cd;
       float d[8], v[8];
       unpack<T, 8>(cd, d);
       if (active) {
         T* dz = static_cast<T*>(a.dz) + r * a.N + zc;
-        unpack<__half, 8>(cz, v);
-        v_mul<8>(v, v, sz);
+        kept_z(cz, cez, v);
         if constexpr (GATED) {
           float u[8], du[8];
-          unpack<__half, 8>(cu, u);
-          v_mul<8>(u, u, su);
+          kept_z(cu, ceu, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float q = sigmoid_f(v[j]);
@@ -1001,9 +1028,13 @@ constexpr int JOIN_TOKENS = 4;
 // z of column c, by a warp that has 32 columns of the row, those that a byte of exponents is for.
 __device__ __forceinline__ void keep_z(const b200_linear_args& la, size_t row, int c, bool in, float z) {
   const uint32_t bits = __float_as_uint(fabsf(z));
-  const int E = shared_exponent(__reduce_max_sync(0xffffffffu, in && bits < 0x7f800000u ? bits : 0u));
+  int E = shared_exponent(__reduce_max_sync(0xffffffffu, in && bits < 0x7f800000u ? bits : 0u));
+  if (E >= 137 && z_spans_much(E, __uint_as_float(__reduce_min_sync(0xffffffffu, in && bits != 0u && bits < 0x7f800000u ? bits : 0x7f7fffffu)))) E = Z_BF16;
   if ((threadIdx.x & 31) == 0 && in) la.zexp[row * zexp_pitch(la.N) + c / 32] = static_cast<unsigned char>(E);
-  if (in) static_cast<__half*>(la.z)[row * la.N + c] = __float2half_rn(z * z_scale(E));
+  if (!in) return;
+  const size_t i = row * la.N + c;
+  if (E != Z_BF16) static_cast<__half*>(la.z)[i] = __float2half_rn(z * z_scale(E));
+  else static_cast<__nv_bfloat16*>(la.z)[i] = __float2bfloat16_rn(z);
 }
 template <int MODE, int TT, typename T>
 __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_linear_args la, int ctas, int quads) {

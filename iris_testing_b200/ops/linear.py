@@ -109,8 +109,8 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
 
 
 def _forward(x, w, bias, residual, group_rows, act, save):
-    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain.  z is fp16 [M, N] and a byte of exponent for every
-    32 columns of a row."""
+    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain.  z is [M, N] of fp16 under a power of two, or of bf16,
+    and a byte for every 32 columns of a row that says which."""
     M, K = x.shape
     G, N = (1, w.shape[0]) if w.dim() == 2 else w.shape[:2]
     n_out = N // 2 if act == 4 else N
@@ -195,7 +195,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
                 and the gradients of x and residual are zero there.
 
     All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
-    the pre-activation is kept to 11 bits and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
+    the pre-activation is kept to 11 bits and to 2^-30 (to 8 bits where 32 neighbouring ones hold both a value of 1024 or
+    more and one 2^31 times smaller) and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
     timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.
     Derivatives are reverse mode, of first order.  CPU tensors take plain PyTorch."""
     if activation not in ACTIVATIONS:
