@@ -35,6 +35,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "elementwise.cuh"
 #include "launch.h"
@@ -50,7 +51,10 @@ typedef struct b200_linear_args {
   void* z;                  // forward: [M, N] of 16 bits or null: fp16 under the powers of two of zexp, or bf16
   unsigned char* zexp;      // with z: [M][ceil(N / 256) * 8], exponents of 32 columns each
   const void* bias;         // [G, N] or null
-  const void* res;          // [M, n_out] or null
+  union {
+    const void* res;            // forward: [M, n_out] or null
+    const unsigned int* peak;   // dX, dW: what dz is under a power of two by (see dz_shift), or null: it is as it is
+  };
   const int* group_rows;    // [G] or null: one group of all M rows
   int* status;
   unsigned long long wait_budget_ns;
@@ -72,6 +76,7 @@ typedef struct b200_act_grad_args {
   void* dbias;              // [G, N] or null
   float* record;            // [chunks + G][N] sums over the rows of a group in a chunk
   const int* group_rows;
+  unsigned int* peak;       // fp16 with an activation: [1], left for the products of dz
   int G, M, N, n_out, elem, act;
   int chunks, chunk_rows;
 } b200_act_grad_args;
@@ -158,6 +163,19 @@ __device__ __forceinline__ float z_scale(int E) { return __uint_as_float(static_
 __device__ __forceinline__ float z_unscale(int E) { return __uint_as_float(static_cast<uint32_t>(E - 14) << 23); }    // 2^(E - 141)
 __device__ __forceinline__ bool z_spans_much(int E, float smallest) { return E >= 137 && smallest * z_scale(E) < 0x1p-17f; }
 __device__ __forceinline__ long long zexp_pitch(int N) { return (N + 255) / 256 * 8; }
+
+// dz of fp16 products: the tensor cores take it in 16 bits like the weights and x that it is multiplied with, off by 2^-11 |dz|
+// and 2^-25 in absolute terms.  (Of bf16, by 2^-8 |dz| at any size.)  Where a call's largest finite |dz| (its fp32 bits are `peak`)
+// would round to infinity, or is below 2^-10, so that what is lost below 2^-25 would count, dz is multiplied with the power of two that
+// takes the largest into [2^14, 2^15), and the products are multiplied back before they are rounded.  Returned is the power's
+// negative exponent.  It stays at 10 at most: a single value of 2^26 may not take the bits of all others.
+constexpr float DZ_LARGEST = 65520.f;      // rounds to infinity
+__device__ __forceinline__ int dz_shift(unsigned int peak) {
+  const int E = static_cast<int>(peak >> 23);
+  if (__uint_as_float(peak) >= DZ_LARGEST) return min(E - 141, 10);
+  return peak != 0u && E < 117 ? max(E - 141, -100) : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 __device__ __forceinline__ uint32_t pack_16(float lo, float hi, bool bf16) {
   if (bf16) return pack_bf16x2(lo, hi);
@@ -462,6 +480,9 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     uint8_t* boxes = staging + q * S::BOXES * LIN_BOX;
     int ring = 0;                                      // the next box
     const bool save_z = MODE == LIN_FORWARD && la.z != nullptr;
+    float unshift = 1.f;
+    if constexpr (MODE != LIN_FORWARD)
+      if (la.peak != nullptr) unshift = power_of_two(dz_shift(*la.peak));
     auto take_box = [&]() {
       uint8_t* box = boxes + ring * LIN_BOX;
       ring = ring + 1 == S::BOXES ? 0 : ring + 1;
@@ -508,7 +529,10 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0u;
           }
-          if constexpr (MODE == LIN_FORWARD) {
+          if constexpr (MODE != LIN_FORWARD) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * unshift);
+          } else {
             const int zcol = n * LBN + cc;             // column of z (of the gate half)
             auto add_bias = [&](uint32_t (&x)[32], int col) {
 #pragma unroll
@@ -662,6 +686,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   }
 }
 
+// The larger magnitude, of finite ones.
+__device__ __forceinline__ float finite_max(float top, float v) {
+  v = fabsf(v);
+  return v <= 3.402823466e38f ? fmaxf(top, v) : top;
+}
 // Eight values of z as they were kept.
 __device__ __forceinline__ void kept_z(const Pack<__half, 8>& k, int e, float (&v)[8]) {
   if (e == Z_BF16) {
@@ -675,11 +704,20 @@ __device__ __forceinline__ void kept_z(const Pack<__half, 8>& k, int e, float (&
 // dz = act'(z) dy and the column sums of dz over each group.  A thread takes eight columns of the output down a run of
 // rows, the next row under way while it works on one; the sums of a (run, group) go to record run + group (both only ever
 // advance), added up in order by the next kernel.  Bound by memory traffic with SUMS off; 64 registers, so that an SM holds
-// 1024 threads.
-template <typename T, bool GATED, bool SUMS>
+// 1024 threads.  fp16: the largest |dz| is found on the way; AGAIN, launched behind it, ends at once as a rule, and otherwise
+// writes dz once more under the power of two that it asks for.
+template <typename T, bool GATED, bool SUMS, bool AGAIN>
 __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_args a) {
   using P = Pack<T, 8>;
   using Z = Pack<__half, 8>;
+  constexpr bool PEAK = std::is_same<T, __half>::value && !AGAIN;
+  float shift = 1.f, top = 0.f;
+  if constexpr (AGAIN) {
+    chain_wait();
+    const int s = dz_shift(*a.peak);
+    if (s == 0) return;
+    shift = power_of_two(-s);
+  }
   // of the gated form, a thread's columns belong to eight columns of the gate and of the up half
   const int oc = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (oc >= a.n_out) return;
@@ -739,11 +777,18 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
             du[j] = d[j] * (q * v[j]);
             d[j] *= u[j] * silu_slope(v[j], q);
             if constexpr (SUMS) sum2[j] += du[j];
+            if constexpr (PEAK) top = finite_max(top, du[j]);
+            if constexpr (AGAIN) du[j] *= shift;
           }
           store_pack<T, 8>(dz + 128, du);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[j] *= act_slope(v[j], a.act);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (PEAK) top = finite_max(top, d[j]);
+          if constexpr (AGAIN) d[j] *= shift;
         }
         store_pack<T, 8>(dz, d);
       }
@@ -765,6 +810,12 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
   if (a.dres != nullptr) {
     const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (long long r = pos; r < r1; ++r) store_pack<T, 8>(static_cast<T*>(a.dres) + r * a.n_out + oc, none);
+  }
+  if constexpr (PEAK) {
+    if (active) {
+      const unsigned int here = __activemask(), most = __reduce_max_sync(here, __float_as_uint(top));
+      if ((threadIdx.x & 31) == __ffs(here) - 1 && most != 0u) atomicMax(a.peak, most);
+    }
   }
 }
 
@@ -1054,6 +1105,7 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
   const int tiles = g_sched_start[la.G] * FT;
   const long long units = static_cast<long long>(tiles) * KB, quota = rows_quota(units, ctas);
   const bool gated = MODE == LIN_FORWARD && la.act == ACT_SILU_GATE;
+  const float unshift = MODE != LIN_FORWARD && la.peak != nullptr ? power_of_two(dz_shift(*la.peak)) : 1.f;
   const long long jobs = static_cast<long long>(tiles) * quads;
   int cursor = 0;
   for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
@@ -1112,6 +1164,8 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
           if (la.z != nullptr) keep_z(la, row, c, in, o);
           o = act_value(o, la.act);
           if (la.res != nullptr && in) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + c]);
+        } else {
+          o *= unshift;
         }
         if (in) y[row * la.n_out + c] = from_f32<T>(o);
       }
@@ -1253,11 +1307,23 @@ template <typename T>
 static cudaError_t act_grad_launch(const b200_act_grad_args& a, cudaStream_t st) {
   const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
   const bool gated = a.act == ACT_SILU_GATE, sums = a.dbias != nullptr;
-  auto kern = gated ? (sums ? act_grad_kernel<T, true, true> : act_grad_kernel<T, true, false>)
-                    : (sums ? act_grad_kernel<T, false, true> : act_grad_kernel<T, false, false>);
+  auto kern = gated ? (sums ? act_grad_kernel<T, true, true, false> : act_grad_kernel<T, true, false, false>)
+                    : (sums ? act_grad_kernel<T, false, true, false> : act_grad_kernel<T, false, false, false>);
+  if (a.peak != nullptr) {
+    const cudaError_t e = cudaMemsetAsync(a.peak, 0, sizeof(unsigned int), st);
+    if (e != cudaSuccess) return e;
+  }
   b200_count_launches(1);
   kern<<<grid, 128, 0, st>>>(a);
   return cudaGetLastError();
+}
+// dz under its power of two, where it needs one.
+static cudaError_t act_grad_again(b200_act_grad_args a, cudaStream_t st) {
+  const dim3 grid(a.chunks, (a.n_out / 8 + 127) / 128);
+  a.dres = nullptr;
+  b200_count_launches(1);
+  return a.act == ACT_SILU_GATE ? launch_chained(act_grad_kernel<__half, true, false, true>, grid, dim3(128), 0, st, a)
+                                : launch_chained(act_grad_kernel<__half, false, false, true>, grid, dim3(128), 0, st, a);
 }
 
 }  // namespace b200
@@ -1274,6 +1340,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
   if (gated && la.N % 256 != 0) return -13;
   if ((la.z != nullptr) != (la.zexp != nullptr)) return -17;
+  if (la.mode != LIN_FORWARD && la.peak != nullptr && la.elem != ELEM_F16) return -18;
   if (la.n_out != (la.mode != LIN_FORWARD ? la.K : gated ? la.N / 2 : la.N)) return -14;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (la.record != nullptr) {
@@ -1311,15 +1378,17 @@ int b200_act_grad(const b200_act_grad_args* args, void* stream) {
   if ((args->act != ACT_NONE) != (args->z != nullptr) || (args->z != nullptr) != (args->dz != nullptr)) return -12;
   if (args->elem != ELEM_BF16 && args->elem != ELEM_F16) return -13;
   if ((args->z != nullptr) != (args->zexp != nullptr)) return -14;
+  if ((args->peak != nullptr) != (args->z != nullptr && args->elem == ELEM_F16)) return -15;
   const b200_act_grad_args& a = *args;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t launched = a.elem == ELEM_BF16 ? act_grad_launch<__nv_bfloat16>(a, st) : act_grad_launch<__half>(a, st);
-  if (launched != cudaSuccess || a.dbias == nullptr) return static_cast<int>(launched);
-  b200_count_launches(1);
-  const dim3 fin((a.N + 31) / 32, a.G);
-  cudaError_t e;
-  if (a.elem == ELEM_BF16) e = launch_chained(bias_grad_kernel<__nv_bfloat16>, fin, dim3(256), 0, st, a);
-  else e = launch_chained(bias_grad_kernel<__half>, fin, dim3(256), 0, st, a);
+  cudaError_t e = a.elem == ELEM_BF16 ? act_grad_launch<__nv_bfloat16>(a, st) : act_grad_launch<__half>(a, st);
+  if (e == cudaSuccess && a.dbias != nullptr) {
+    b200_count_launches(1);
+    const dim3 fin((a.N + 31) / 32, a.G);
+    e = a.elem == ELEM_BF16 ? launch_chained(bias_grad_kernel<__nv_bfloat16>, fin, dim3(256), 0, st, a)
+                            : launch_chained(bias_grad_kernel<__half>, fin, dim3(256), 0, st, a);
+  }
+  if (e == cudaSuccess && a.peak != nullptr) e = act_grad_again(a, st);
   return static_cast<int>(e);
 }
 

@@ -37,7 +37,7 @@ class LinearArgs(C.Structure):
 
 
 class ActGradArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "zexp", "dz", "dres", "dbias", "record", "group_rows")] \
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "z", "zexp", "dz", "dres", "dbias", "record", "group_rows", "peak")] \
         + [(n, C.c_int) for n in ("G", "M", "N", "n_out", "elem", "act", "chunks", "chunk_rows")]
 
 
@@ -84,7 +84,7 @@ def _record_floats(mode: int, M: int, N: int, K: int, G: int, sms: int) -> int:
     return declare("b200_linear_record_floats", [C.c_int] * 6, C.c_longlong)(mode, M, N, K, G, sms)
 
 
-def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, res=None):
+def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, res=None, peak=None):
     la = LinearArgs()
     la.a, la.b, la.out = a.data_ptr(), b.data_ptr(), out.data_ptr()
     if z is not None:
@@ -95,6 +95,8 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
         la.res = res.data_ptr()
     if group_rows is not None:
         la.group_rows = group_rows.data_ptr()
+    if peak is not None:
+        la.res = peak.data_ptr()             # in the residual's place
     la.status = launch_status(a.device).data_ptr()
     la.wait_budget_ns = 2_000_000_000
     la.mode, la.G, la.M, la.N, la.K, la.n_out = mode, G, M, N, K, out.shape[-1]
@@ -140,12 +142,15 @@ def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
     own_dres = dres is not None and dres is not dy
     slope = act and (db is not None or dx is not None or dw is not None)      # act'(z) has a part in what is asked for
     with on_device(x):
-        dz = dy
+        dz, peak = dy, None
         if db is not None or own_dres or slope:
             a = ActGradArgs()
             if slope:
                 dz = torch.empty((M, N), dtype=dt, device=dev)
                 a.z, a.zexp, a.dz, a.act = z[0].data_ptr(), z[1].data_ptr(), dz.data_ptr(), act
+                if dt == torch.float16:
+                    peak = torch.empty(1, dtype=torch.int32, device=dev)
+                    a.peak = peak.data_ptr()
             a.dy = dy.data_ptr()
             a.dres = dres.data_ptr() if own_dres else None
             a.G, a.M, a.N, a.n_out, a.elem = G, M, dz.shape[1], dy.shape[1], ELEM[dt]
@@ -157,9 +162,9 @@ def _backward(x, w, z, has_bias, has_res, group_rows, act, need, dy):
                 a.dbias, a.record = db.data_ptr(), record.data_ptr()
             _ACT_GRAD(a, stream_ptr(x))
         if dx is not None:
-            _product(_DX, dz, w, dx, M, N, K, G, group_rows)
+            _product(_DX, dz, w, dx, M, N, K, G, group_rows, peak=peak)
         if dw is not None:
-            _product(_DW, dz, x, dw, M, N, K, G, group_rows)
+            _product(_DW, dz, x, dw, M, N, K, G, group_rows, peak=peak)
     return dx, dw, db, dres
 
 
@@ -196,7 +201,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
 
     All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
     the pre-activation is kept to 11 bits and to 2^-30 (to 8 bits where 32 neighbouring ones hold both a value of 1024 or
-    more and one 2^31 times smaller) and its gradient in x's dtype.  Groups that hold more rows than x has, and device-side
+    more and one 2^31 times smaller), and its gradient dz in x's dtype; that of fp16 under a power of two for the whole call, up
+    to 2^10, where the largest |dz| is above 65504 or below 2^-10.  Groups that hold more rows than x has, and device-side
     timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.
     Derivatives are reverse mode, of first order.  CPU tensors take plain PyTorch."""
     if activation not in ACTIVATIONS:

@@ -102,7 +102,7 @@ def test_gradients_to_11_bits_of_z(rows, N, K, act, dtype):
 @pytest.mark.parametrize("split", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ACTS[1:])
-@pytest.mark.parametrize("size", [2.0 ** 9, 2.0 ** 12, 2.0 ** 27, 1e10, 1e12, 1e13, 1e20])
+@pytest.mark.parametrize("size", [2.0 ** 9, 2.0 ** 12, 2.0 ** 27, 2.0 ** 31, 1e10, 1e12, 1e13, 1e20])
 def test_gradients_next_to_a_large_value(size, act, dtype, split, monkeypatch):
     """One column of 32 holds a value that leaves ordinary ones far behind: their slopes and, of the gated form, the products with
     them are as right as without it."""
