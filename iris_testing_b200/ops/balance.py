@@ -151,6 +151,8 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
         raise ValueError(f"at most {MAX_BALANCE_EXPERTS} experts (got {E})")
     if T > MAX_TOKENS or (seq_rows is not None and seq_rows.numel() * -(-E // 32) > MAX_TOKENS):
         raise ValueError(f"at most {MAX_TOKENS} tokens, and blocks of 32 experts of all sequences")
+    if topk_idx.shape[1] > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} experts of a token")
     require_device(logits.device, topk_idx=topk_idx, seq_rows=seq_rows, token_mask=token_mask)
     refuse_tangents(logits=logits)
     logits, idx = rows_view(logits), topk_idx.contiguous()

@@ -19,6 +19,7 @@ from .expert import pairs_pay, sm_count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "silu_gate": 4}
 _FORWARD, _DX, _DW = 0, 1, 2
+MAX_GRAD_COLUMNS = 65535 * 1024  # blocks side by side in the activation's gradient, of 1024 columns each
 MAX_ROWS = 2 ** 31 - 1024        # a last tile that is partly empty still has row numbers of 32 bits
 
 
@@ -233,8 +234,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     require(w_kmajor.dtype == dt and (bias is None or bias.dtype == dt) and (residual is None or residual.dtype == dt),
             "w_kmajor, bias and residual must have x's dtype")
     require(K % 8 == 0 and N % 8 == 0, "K and N must be multiples of 8")
-    if x.numel() // K > MAX_ROWS or G * N > MAX_ROWS:
-        raise ValueError(f"at most {MAX_ROWS} rows of x, and of the weights of all groups")
+    if x.numel() // K > MAX_ROWS or G * N > MAX_ROWS or K > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows of x and of the weights of all groups, and columns")
     require_device(x.device, w_kmajor=w_kmajor, bias=bias, residual=residual, group_rows=group_rows)
     refuse_tangents(x=x, w_kmajor=w_kmajor, bias=bias, residual=residual)
     flat = len(shape) == 2                   # no views, which autograd would have to pass through
@@ -243,6 +244,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     w, b, r2 = _plain(w_kmajor), _plain(bias), _plain(r2)
     rows = None if group_rows is None else group_rows.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_kmajor, bias, residual)):
+        if n_out > MAX_GRAD_COLUMNS and (act or b is not None or (grouped and r2 is not None)):
+            raise ValueError(f"at most {MAX_GRAD_COLUMNS} columns of the result with gradients")
         y = _Linear.apply(x2, w, b, r2, rows, act)
     else:
         y, _ = _forward(x2, w, b, r2, rows, act, False)
