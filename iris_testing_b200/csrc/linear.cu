@@ -19,12 +19,14 @@
 // block is loaded first and multiplied third, which hides the mending (64 groups of 1023 rows: 612 us, 631 when it came last;
 // 603 for 1024 rows, which need none).
 //
-// The pre-activations z are kept for the backward pass as fp16 under a power of two that 32 columns of a row share, kept in a
-// byte: off by 2^-11 |z|, and by 2^-30 in absolute terms.  fp16 spans too little for 32 columns that hold both a value of
+// The pre-activations z are kept for the backward pass, of bf16 products as fp16 under a power of two that 32 columns of a row share,
+// kept in a byte: off by 2^-11 |z|, and by 2^-30 in absolute terms.  fp16 spans too little for 32 columns that hold both a value of
 // 1024 or more and one 2^31 times smaller than it: those are kept as bf16, off by 2^-8 |z| whatever the size (beside
 // 1e12, a 1 under a shared power of two would be kept as nothing, and its slope and its products with it).  (Kept as bf16
 // throughout, dX and dW of a gated bf16 product are 3.0e-3 off instead of 2.4e-3, relative; 1.7e-3 is what rounding the result
-// alone costs.)
+// alone costs.)  Of fp16 products z is the upper 24 bits of the fp32 sum, 16 of them in z and a byte beside it: off by 2^-15 |z|.
+// (With 11 bits, dX and dW of a gated fp16 product were 3.7e-4 off instead of 3.0e-4, which is what rounding dz and the result costs;
+// the result alone 2.1e-4.)
 // dz is rounded to the element type, since the tensor cores multiply 16-bit values: at most half a step of each value, which
 // averages out over the contracted dimension.
 #include <cuda.h>
@@ -48,8 +50,8 @@ typedef struct b200_linear_args {
   const void* a;            // forward: x [M, K]; dX: dz [M, N]; dW: dz [M, N]
   const void* b;            // forward, dX: W [G, N, K]; dW: x [M, K]
   void* out;                // y [M, n_out]; dx [M, K]; dW [G, N, K]
-  void* z;                  // forward: [M, N] of 16 bits or null: fp16 under the powers of two of zexp, or bf16
-  unsigned char* zexp;      // with z: [M][ceil(N / 256) * 8], exponents of 32 columns each
+  void* z;                  // forward: [M, N] of 16 bits or null; what they are, zexp says
+  unsigned char* zexp;      // with z, bf16: [M][ceil(N / 256) * 8], exponents of 32 columns each; fp16: [M][ceil(N / 256) * 256], z's next 8 bits
   const void* bias;         // [G, N] or null
   union {
     const void* res;            // forward: [M, n_out] or null
@@ -152,7 +154,7 @@ __device__ __forceinline__ float act_slope(float v, int act) {
   return q * fmaf(v * fmaf(3.f * GELU_B, vv, GELU_A), 1.f - q, 1.f);
 }
 
-// z in fp16 under a shared power of two: E is the largest finite magnitude's exponent (biased, 15 at least), the
+// z of bf16 products, in fp16 under a shared power of two: E is the largest finite magnitude's exponent (biased, 15 at least), the
 // values are scaled into [0, 2^15], where fp16 has 11 bits down to 2^-14, 8 down to 2^-17 and an absolute error of 2^-25.
 // Infinities and NaN stay what they are; so near to fp32's largest value that rounding reaches 2^128, z becomes infinite.
 // Scales of 2^-5 and below (E >= 137: a value of 1024) leave an absolute error that ordinary values may feel: there, where the
@@ -163,6 +165,13 @@ __device__ __forceinline__ float z_scale(int E) { return __uint_as_float(static_
 __device__ __forceinline__ float z_unscale(int E) { return __uint_as_float(static_cast<uint32_t>(E - 14) << 23); }    // 2^(E - 141)
 __device__ __forceinline__ bool z_spans_much(int E, float smallest) { return E >= 137 && smallest * z_scale(E) < 0x1p-17f; }
 __device__ __forceinline__ long long zexp_pitch(int N) { return (N + 255) / 256 * 8; }
+// Of fp16 products: the upper 16 bits of fp32 values beside each other, and the 8 bits below of four values.  (Cut, not
+// rounded, so that infinities and NaN stay what they are.)
+__device__ __forceinline__ long long zlow_pitch(int N) { return (N + 255) / 256 * 256; }
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ uint32_t lower_bytes(const uint32_t* x) {
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0051), __byte_perm(x[2], x[3], 0x0051), 0x5410);
+}
 
 // dz of fp16 products: the tensor cores take it in 16 bits like the weights and x that it is multiplied with, off by 2^-11 |dz|
 // and 2^-25 in absolute terms.  (Of bf16, by 2^-8 |dz| at any size.)  Where a call's largest finite |dz| (its fp32 bits are `peak`)
@@ -243,7 +252,8 @@ __device__ __forceinline__ void store_box(const uint8_t* box, const CUtensorMap*
   if (lane == 0) bulk_commit_group();
 }
 
-template <int MODE, int CG, bool GATED>
+// Z24: how z is kept, of fp16 products (forward).
+template <int MODE, int CG, bool GATED, bool Z24>
 __global__ void __launch_bounds__(LIN_THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
               const __grid_constant__ CUtensorMap tmap_o, const __grid_constant__ CUtensorMap tmap_z, const b200_linear_args la) {
@@ -554,6 +564,21 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             }
             if (save_z) {
               auto put = [&](const uint32_t (&x)[32], uint8_t* box, int col, int chunk) {
+                if constexpr (Z24) {
+                  uint32_t low[8];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) low[i] = lower_bytes(x + 4 * i);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + i) ^ (lane & 7)) << 4)) =
+                        make_uint4(upper_halves(x[8 * i], x[8 * i + 1]), upper_halves(x[8 * i + 2], x[8 * i + 3]),
+                                   upper_halves(x[8 * i + 4], x[8 * i + 5]), upper_halves(x[8 * i + 6], x[8 * i + 7]));
+                  if (!row_ok) return;
+                  uint4* bytes = reinterpret_cast<uint4*>(la.zexp + (row0 + lane) * zlow_pitch(la.N) + col);
+                  bytes[0] = make_uint4(low[0], low[1], low[2], low[3]);
+                  bytes[1] = make_uint4(low[4], low[5], low[6], low[7]);
+                  return;
+                }
                 float m = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -634,7 +659,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             store_box(ubox, &tmap_z, static_cast<char*>(la.z), ldz, row0, n * LBN + LBN / 2 + p * 64, la.N, rows_here, lane);
         }
       }
-      if (save_z && row_ok)
+      if (!Z24 && save_z && row_ok)
         *reinterpret_cast<unsigned long long*>(la.zexp + (row0 + lane) * zexp_pitch(la.N) + n * 8) = exponents;
     }
     if (lane == 0) bulk_wait_group<0>();               // shared memory stays allocated until the stores are done
@@ -691,15 +716,43 @@ __device__ __forceinline__ float finite_max(float top, float v) {
   v = fabsf(v);
   return v <= 3.402823466e38f ? fmaxf(top, v) : top;
 }
-// Eight values of z as they were kept.
-__device__ __forceinline__ void kept_z(const Pack<__half, 8>& k, int e, float (&v)[8]) {
-  if (e == Z_BF16) {
-    unpack<__nv_bfloat16, 8>(*reinterpret_cast<const Pack<__nv_bfloat16, 8>*>(&k), v);
-  } else {
-    unpack<__half, 8>(k, v);
-    v_mul<8>(v, v, z_unscale(e));
+// Eight values of z as they were kept, with what belongs to them beside z.
+template <typename T>
+struct ZBeside;
+template <>
+struct ZBeside<__nv_bfloat16> {
+  int e = 141;
+  static __device__ __forceinline__ long long pitch(int N) { return zexp_pitch(N); }
+  static __device__ __forceinline__ int column(int c) { return c / 32; }
+  __device__ __forceinline__ void load(const unsigned char* p) { e = *p; }
+  __device__ __forceinline__ void values(const Pack<__half, 8>& k, float (&v)[8]) const {
+    if (e == Z_BF16) {
+      unpack<__nv_bfloat16, 8>(*reinterpret_cast<const Pack<__nv_bfloat16, 8>*>(&k), v);
+    } else {
+      unpack<__half, 8>(k, v);
+      v_mul<8>(v, v, z_unscale(e));
+    }
   }
-}
+};
+template <>
+struct ZBeside<__half> {
+  uint2 low = {0u, 0u};
+  static __device__ __forceinline__ long long pitch(int N) { return zlow_pitch(N); }
+  static __device__ __forceinline__ int column(int c) { return c; }
+  __device__ __forceinline__ void load(const unsigned char* p) { low = *reinterpret_cast<const uint2*>(p); }
+  // the byte stands for the last eight bits as well, which leaves 0 and all numbers of 16 bits as they are
+  __device__ __forceinline__ void values(const Pack<__half, 8>& k, float (&v)[8]) const {
+    const uint4 w = *reinterpret_cast<const uint4*>(&k);
+    v[0] = __uint_as_float(__byte_perm(w.x, low.x, 0x1044));
+    v[1] = __uint_as_float(__byte_perm(w.x, low.x, 0x3255));
+    v[2] = __uint_as_float(__byte_perm(w.y, low.x, 0x1066));
+    v[3] = __uint_as_float(__byte_perm(w.y, low.x, 0x3277));
+    v[4] = __uint_as_float(__byte_perm(w.z, low.y, 0x1044));
+    v[5] = __uint_as_float(__byte_perm(w.z, low.y, 0x3255));
+    v[6] = __uint_as_float(__byte_perm(w.w, low.y, 0x1066));
+    v[7] = __uint_as_float(__byte_perm(w.w, low.y, 0x3277));
+  }
+};
 
 // dz = act'(z) dy and the column sums of dz over each group.  A thread takes eight columns of the output down a run of
 // rows, the next row under way while it works on one; the sums of a (run, group) go to record run + group (both only ever
@@ -730,8 +783,9 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
   const T* dy = static_cast<const T*>(a.dy) + oc;
   const __half* z = static_cast<const __half*>(a.z) + zc;
   const bool active = a.z != nullptr;
-  const unsigned char* zexp = a.zexp + zc / 32;            // gated: the up half's four bytes on
-  const long long pitch = zexp_pitch(a.N);
+  using Beside = ZBeside<T>;
+  const unsigned char* zexp = a.zexp + Beside::column(zc);
+  const long long pitch = Beside::pitch(a.N);
   long long pos = first;
   for (; g < a.G && pos < r1; ++g) {
     const long long end = min(r1, start + rows_of(g));
@@ -744,33 +798,33 @@ __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_ar
     }
     P kd;
     Z kz, ku;
-    int ez = 141, eu = 141;
+    Beside ez, eu;
     auto load = [&](long long r) {
       kd = *reinterpret_cast<const P*>(dy + r * a.n_out);
       if (active) {
         kz = *reinterpret_cast<const Z*>(z + r * a.N);
-        ez = zexp[r * pitch];
+        ez.load(zexp + r * pitch);
       }
       if (GATED) {
         ku = *reinterpret_cast<const Z*>(z + r * a.N + 128);
-        eu = zexp[r * pitch + 4];
+        eu.load(zexp + r * pitch + Beside::column(128));
       }
     };
     load(pos);
     for (long long r = pos; r < end; ++r) {
       const P cd = kd;
       const Z cz = kz, cu = ku;
-      const int cez = ez, ceu = eu;
+      const Beside cez = ez, ceu = eu;
       if (r + 1 < end) load(r + 1);
       if (a.dres != nullptr) *reinterpret_cast<P*>(static_cast<T*>(a.dres) + r * a.n_out + oc) = cd;
       float d[8], v[8];
       unpack<T, 8>(cd, d);
       if (active) {
         T* dz = static_cast<T*>(a.dz) + r * a.N + zc;
-        kept_z(cz, cez, v);
+        cez.values(cz, v);
         if constexpr (GATED) {
           float u[8], du[8];
-          kept_z(cu, ceu, u);
+          ceu.values(cu, u);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float q = sigmoid_f(v[j]);
@@ -1077,7 +1131,14 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 // (gated: an output of two of them).
 constexpr int JOIN_TOKENS = 4;
 // z of column c, by a warp that has 32 columns of the row, those that a byte of exponents is for.
+template <typename T>
 __device__ __forceinline__ void keep_z(const b200_linear_args& la, size_t row, int c, bool in, float z) {
+  if constexpr (std::is_same<T, __half>::value) {
+    if (!in) return;
+    static_cast<unsigned short*>(la.z)[row * la.N + c] = static_cast<unsigned short>(__float_as_uint(z) >> 16);
+    la.zexp[row * zlow_pitch(la.N) + c] = static_cast<unsigned char>(__float_as_uint(z) >> 8);
+    return;
+  }
   const uint32_t bits = __float_as_uint(fabsf(z));
   int E = shared_exponent(__reduce_max_sync(0xffffffffu, in && bits < 0x7f800000u ? bits : 0u));
   if (E >= 137 && z_spans_much(E, __uint_as_float(__reduce_min_sync(0xffffffffu, in && bits != 0u && bits < 0x7f800000u ? bits : 0x7f7fffffu)))) E = Z_BF16;
@@ -1143,8 +1204,8 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
         if (!have[2 * j]) continue;
         const size_t row = row0 + k + 2 * j;
         if (la.z != nullptr) {
-          keep_z(la, row, zc, true, v[2 * j]);
-          keep_z(la, row, zc + 128, true, v[2 * j + 1]);
+          keep_z<T>(la, row, zc, true, v[2 * j]);
+          keep_z<T>(la, row, zc + 128, true, v[2 * j + 1]);
         }
         float o = gated_value(v[2 * j], v[2 * j + 1]);
         if (la.res != nullptr) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + yc]);
@@ -1161,7 +1222,7 @@ __global__ void __launch_bounds__(ROWS_FEATURES) linear_join_kernel(const b200_l
         float o = v[j];
         if constexpr (MODE == LIN_FORWARD) {
           o += b;
-          if (la.z != nullptr) keep_z(la, row, c, in, o);
+          if (la.z != nullptr) keep_z<T>(la, row, c, in, o);
           o = act_value(o, la.act);
           if (la.res != nullptr && in) o += to_f32(static_cast<const T*>(la.res)[row * la.n_out + c]);
         } else {
@@ -1208,11 +1269,11 @@ static int lin_map(CUtensorMap* tm, const void* base, int elem, long long planes
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-template <int MODE, int CG, bool GATED>
+template <int MODE, int CG, bool GATED, bool Z24 = false>
 static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) {
   static std::atomic<unsigned long long> configured{0};
   using S = LinGeo<MODE, CG>;
-  auto kern = linear_kernel<MODE, CG, GATED>;
+  auto kern = linear_kernel<MODE, CG, GATED, Z24>;
   constexpr int smem = lin_smem<MODE, CG>();
   // The device's context becomes current: the thread that runs a backward pass may not have met it yet, and tensor maps
   // are encoded by the CUDA driver, which does not do so itself.
@@ -1249,6 +1310,12 @@ static int linear_launch(const b200_linear_args& la, int ctas, cudaStream_t st) 
   cfg.numAttrs = 1;
   b200_count_launches(1);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, ta, tb, to, tz, la));
+}
+
+template <bool Z24>
+static int linear_forward(const b200_linear_args& la, bool gated, int ctas, cudaStream_t st) {
+  if (gated) return la.pair ? linear_launch<LIN_FORWARD, 2, true, Z24>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, true, Z24>(la, ctas, st);
+  return la.pair ? linear_launch<LIN_FORWARD, 2, false, Z24>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, false, Z24>(la, ctas, st);
 }
 
 // Tokens of a tile: as few as hold an average group.
@@ -1339,7 +1406,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   if ((la.group_rows == nullptr && la.G != 1) || la.M > LIN_MAX_ROWS || static_cast<long long>(la.G) * la.N > LIN_MAX_ROWS) return -12;
   const bool gated = la.mode == LIN_FORWARD && la.act == ACT_SILU_GATE;
   if (gated && la.N % 256 != 0) return -13;
-  if ((la.z != nullptr) != (la.zexp != nullptr)) return -17;
+  if ((la.z != nullptr) != (la.zexp != nullptr) || (reinterpret_cast<uintptr_t>(la.zexp) & 15u) != 0) return -17;
   if (la.mode != LIN_FORWARD && la.peak != nullptr && la.elem != ELEM_F16) return -18;
   if (la.n_out != (la.mode != LIN_FORWARD ? la.K : gated ? la.N / 2 : la.N)) return -14;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1353,9 +1420,7 @@ int b200_linear(const b200_linear_args* args, int ctas, void* stream) {
   const long long gm = (48ll << 20) / tile_bytes;
   la.group_m = static_cast<int>(gm < 1 ? 1 : gm > 16 ? 16 : gm);
   switch (la.mode) {
-    case LIN_FORWARD:
-      if (gated) return la.pair ? linear_launch<LIN_FORWARD, 2, true>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, true>(la, ctas, st);
-      return la.pair ? linear_launch<LIN_FORWARD, 2, false>(la, ctas, st) : linear_launch<LIN_FORWARD, 1, false>(la, ctas, st);
+    case LIN_FORWARD: return la.elem == ELEM_F16 ? linear_forward<true>(la, gated, ctas, st) : linear_forward<false>(la, gated, ctas, st);
     case LIN_DX: return la.pair ? linear_launch<LIN_DX, 2, false>(la, ctas, st) : linear_launch<LIN_DX, 1, false>(la, ctas, st);
     case LIN_DW: return la.pair ? linear_launch<LIN_DW, 2, false>(la, ctas, st) : linear_launch<LIN_DW, 1, false>(la, ctas, st);
   }

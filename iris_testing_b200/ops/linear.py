@@ -112,8 +112,8 @@ def _product(mode, a, b, out, M, N, K, G, group_rows, act=0, z=None, bias=None, 
 
 
 def _forward(x, w, bias, residual, group_rows, act, save):
-    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain.  z is [M, N] of fp16 under a power of two, or of bf16,
-    and a byte for every 32 columns of a row that says which."""
+    """(y [M, n_out], z or None): x [M, K], w [N, K] or [G, N, K], all plain.  z, for bf16: [M, N] of fp16 under a power of two, or of
+    bf16, and a byte for every 32 columns of a row that says which; for fp16: the upper 16 bits of fp32, and a byte with the next 8."""
     M, K = x.shape
     G, N = (1, w.shape[0]) if w.dim() == 2 else w.shape[:2]
     n_out = N // 2 if act == 4 else N
@@ -121,7 +121,7 @@ def _forward(x, w, bias, residual, group_rows, act, save):
     z = None
     if save and act:
         z = (torch.empty((M, N), dtype=torch.float16, device=x.device),
-             torch.empty((M, -(-N // 256) * 8), dtype=torch.uint8, device=x.device))
+             torch.empty((M, -(-N // 256) * (256 if x.dtype == torch.float16 else 8)), dtype=torch.uint8, device=x.device))
     if M > 0:
         with on_device(x):
             _product(_FORWARD, x, w, y, M, N, K, G, group_rows, act, z, bias, residual)
@@ -201,8 +201,8 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
                 and the gradients of x and residual are zero there.
 
     All of one dtype; K and N are multiples of 8.  Sums are fp32, results are rounded once; for the backward pass
-    the pre-activation is kept to 11 bits and to 2^-30 (to 8 bits where 32 neighbouring ones hold both a value of 1024 or
-    more and one 2^31 times smaller), and its gradient dz in x's dtype; that of fp16 under a power of two for the whole call, up
+    the pre-activation is kept to 16 bits (fp16), or to 11 bits and to 2^-30 (bf16; to 8 bits where 32 neighbouring ones hold
+    both a value of 1024 or more and one 2^31 times smaller), and its gradient dz in x's dtype; that of fp16 under a power of two for the whole call, up
     to 2^10, where the largest |dz| is above 65504 or below 2^-10.  Groups that hold more rows than x has, and device-side
     timeouts, are reported to :func:`check_default_status`.  The same inputs give the same bits.
     Derivatives are reverse mode, of first order.  CPU tensors take plain PyTorch."""

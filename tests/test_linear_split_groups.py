@@ -87,7 +87,7 @@ def test_nothing_is_written_around_the_results(rows, dtype, act, split):
     code = linear.ACTIVATIONS[act]
     ops.check_default_status()
     guard = Guarded()
-    y, z, zexp = guard(dy), guard(torch.empty(M, N, dtype=torch.float16)), guard(torch.empty(M, N // 32, dtype=torch.uint8))
+    y, z, zexp = guard(dy), guard(torch.empty(M, N, dtype=torch.float16)), guard(torch.empty(M, N if dtype == torch.float16 else N // 32, dtype=torch.uint8))
     dx, dw, dz, dres, db = guard(x), guard(w), guard(torch.empty(M, N, dtype=dtype)), guard(dy), guard(b)
     z.zero_()
     zexp.fill_(127)
