@@ -55,7 +55,9 @@ namespace b200 {
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_E = 1024;
 constexpr int BAL_MOST = 0x7fffffff - 0xfffff;      // tokens, and blocks of 32 experts of all sequences: their numbers have 32 bits
-// Blocks of an SM: as many runs as these make no second, half empty round.
+// Blocks of an SM: as many runs as these make no second, half empty round.  (The registers that this leaves, 64 and 80, make the
+// fp32 forms of the forward kernel spill 12 - 20 bytes, its forms for rows off 16 bytes up to 104, and the backward one for fp32
+// rows of 257 experts and more 12.)
 constexpr int BAL_FORWARD_BLOCKS = 4, BAL_BACKWARD_BLOCKS = 3;
 
 template <typename T> __device__ __forceinline__ float lowest();

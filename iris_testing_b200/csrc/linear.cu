@@ -132,7 +132,8 @@ constexpr int lin_smem() {
 static_assert(lin_smem<LIN_FORWARD, 1>() <= 232448 && lin_smem<LIN_FORWARD, 2>() <= 232448 && lin_smem<LIN_DW, 1>() <= 232448 &&
                   lin_smem<LIN_DW, 2>() <= 232448, "exceeds 227 KiB of shared memory per CTA");
 
-// q = 1 / (1 + exp(-v)): relative error a few 2^-22, far below the rounding of a 16-bit result.
+// q = 1 / (1 + exp(-v)): 1 - q, and q where v is negative, are off by up to 2^-21 + 1.3 |v| 2^-24, relative (the rounding of the
+// exponent, log2(e) v, grows with it), which is 2^-17 where fp32 ends.  A 16-bit result is rounded to 2^-11.
 __device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.f + exp2_approx(__fmul_rn(-LOG2_E, v))); }
 constexpr float GELU_A = 2.f * 0.7978845608028654f, GELU_B = GELU_A * 0.044715f;    // tanh form: v * sigmoid(A v + B v^3)
 // The products are rounded before anything is added to them, so that a result does not depend on what else its kernel
@@ -757,8 +758,8 @@ struct ZBeside<__half> {
 // dz = act'(z) dy and the column sums of dz over each group.  A thread takes eight columns of the output down a run of
 // rows, the next row under way while it works on one; the sums of a (run, group) go to record run + group (both only ever
 // advance), added up in order by the next kernel.  Bound by memory traffic with SUMS off; 64 registers, so that an SM holds
-// 1024 threads.  fp16: the largest |dz| is found on the way; AGAIN, launched behind it, ends at once as a rule, and otherwise
-// writes dz once more under the power of two that it asks for.
+// 1024 threads (the gated form with SUMS spills 36 - 56 bytes for that).  fp16: the largest |dz| is found on the way; AGAIN,
+// launched behind it, ends at once as a rule, and otherwise writes dz once more under the power of two that it asks for.
 template <typename T, bool GATED, bool SUMS, bool AGAIN>
 __global__ void __launch_bounds__(128, 8) act_grad_kernel(const b200_act_grad_args a) {
   using P = Pack<T, 8>;

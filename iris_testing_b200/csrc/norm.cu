@@ -61,7 +61,9 @@ constexpr int NORM_WARP_ROWS = 4;      // rows of a block where a warp has a row
 constexpr int NORM_ELEMS = 16;         // elements of a row per thread (8 where that is enough)
 
 // Threads of a block and blocks of an SM of a variant: MAXT is the most threads that share a row (32: a warp).  512
-// threads an SM leave 128 registers each; where 1024 threads share a row (more than 8192 columns) it is 64.  The forward
+// threads an SM leave 128 registers each; where 1024 threads share a row (more than 8192 columns) it is 64, and the backward
+// kernels spill 260 - 440 bytes a thread (4096 rows of 16384 bf16 columns, without / with a next norm: forward 100 / 152 us,
+// backward 185 / 368, for 42 / 83 and 62 / 125 of bytes at the copy rate; nothing is fetched ahead there either).  The forward
 // kernel of 16-bit rows above 4096 and up to 6144 columns needs 78 and so has two blocks of 384 threads on an SM instead of
 // one: 8192 rows of 5120 columns 52 -> 40 us, with a residual 58 -> 48, with a next norm 75 -> 62; of 6144 columns
 // 52 -> 44, 59 -> 56, 77 -> 77.  For fp32 rows the two are even (68 -> 62, 87 -> 93, 122 -> 118), and one block stays.
@@ -71,7 +73,8 @@ template <int MAXT>
 constexpr int NORM_THREADS = MAXT == 32 ? NORM_WARP_ROWS * 32 : MAXT;
 // Rows on their way ahead of the one in work: up to three, by the slots that fit beside each other on an SM (two tensors
 // forward, four and the two column vectors backward); none for the widest rows and for rows that do not lie on 16 bytes,
-// which go straight to registers.
+// which go straight to registers (8192 rows of 4099 columns: forward 207 us, backward 335; of 4096: 32 and 46).  The forms
+// without a next norm have room for w2's factors too, and do not use it.
 constexpr int NORM_SLOT_BYTES = 200 * 1024;
 template <bool BACK, int VEC, int VPT, int MAXT>
 constexpr int NORM_VECTOR_BYTES = BACK && VEC > 1 && MAXT != 1024 ? 2 * VPT * VEC * 4 * NORM_THREADS<MAXT> : 0;

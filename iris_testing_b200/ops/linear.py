@@ -25,7 +25,9 @@ MAX_ROWS = 2 ** 31 - 1024        # a last tile that is partly empty still has ro
 
 def _run_rows(M: int, n_out: int) -> int:
     """Rows that a thread of the activation's gradient goes down: as many as leave 16 blocks for every SM, so that enough
-    loads are under way (64 / 32 rows: 4000 x 14336 77 / 70 us, gated 65536 x 2816 177 / 159)."""
+    loads are under way.  64 / 32 / 16 rows, us, with cold caches, alone: 1000 x 4096 59 / 33 / 23, 8192 x 4096 76 / 53 / 53,
+    4000 x 14336 88 / 90 / 80, gated 65536 x 2816 196 / 176 / 176; with the bias' gradient, whose records shorter runs make
+    more of: 60 / 36 / 24, 79 / 58 / 69, 91 / 95 / 91, 255 / 226 / 241."""
     blocks = -(-n_out // 1024)
     return 64 if M * blocks >= 64 * 2368 else 32 if M * blocks >= 32 * 2368 else 16
 
