@@ -109,3 +109,73 @@ def test_large_gradients(rows, N, K, split, monkeypatch):
         assert torch.isfinite(pair[0]).all() and float(pair[0].abs().max()) < 6e4, "the results are meant to fit"
         within(got.view(t.shape), pair, name)
     ops.check_default_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [[3, 9, 0, 20], [300, 170, 0, 500]])
+def test_the_power_of_two_goes_with_the_inputs_of_a_replay(rows):
+    """Captured with ordinary gradients, replayed with ones that need a power of two, then with smaller ones and with ordinary
+    ones again; two graphs, and another stream, get the same bits as calls without a graph."""
+    from iris_testing_b200 import ops
+    x, w, b, _, dy = inputs(rows, 512, 256, torch.float16, "silu_gate", True, False, "cuda", slack=11)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    gr = torch.tensor(rows, dtype=torch.int32, device="cuda")
+
+    def step():
+        y = ops.linear(*leaves, activation="silu_gate", group_rows=gr)
+        return torch.autograd.grad(y, leaves, dy)
+    first = step()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(step())
+    plain, bx, bw = dy.clone(), x.detach().clone(), w.detach().clone()
+    seen = []
+    for scale, small in ((1.0, 1.0), (2000.0, 2.0 ** -8), (2.0 ** -20, 1.0), (1.0, 1.0)):
+        with torch.no_grad():
+            dy.copy_(plain * scale)
+            x.copy_(bx * small)
+            b.copy_(torch.full_like(b, 100.0) if scale > 1 else torch.full_like(b, 0.25))
+        for g in graphs:
+            g.replay()
+        want = step()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        for out in (*outs, other):
+            for p, q in zip(out, want):
+                assert torch.equal(p, q)
+        # of the second, dx sums 512 products of 2e5 and 1 / 16 and dw up to 500 of 2e5 and 2^-8, up to four times 17000: what is
+        # beyond the type is infinite, and nothing is NaN
+        assert not torch.isnan(want[0]).any() and not torch.isnan(want[1]).any()
+        seen.append(largest(x.detach(), w.detach(), b.detach(), "silu_gate", rows, dy))
+    assert seen[0] == seen[3] and seen[1] > 65520 and seen[2] < 2.0 ** -10 < seen[0] < 65504
+    assert all(t.shape == s.shape for t, s in zip(first, leaves))
+    ops.check_default_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_an_infinite_gradient_stays_in_its_row(bad):
+    """It has no part in the power of two, and reaches no other row or group."""
+    from iris_testing_b200 import ops
+    rows = [70, 33, 0, 100]
+    x, w, b, _, dy = inputs(rows, 256, 128, torch.float16, "silu_gate", True, False, "cuda", slack=9)
+    dy = dy * 2.0 ** -18                                             # small ones, under a power of two
+    gr = torch.tensor(rows, dtype=torch.int32, device="cuda")
+
+    def grads():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        return torch.autograd.grad(ops.linear(*leaves, activation="silu_gate", group_rows=gr), leaves, dy)
+    want = grads()
+    dy[80] = 0
+    dy[203:] = bad                                                   # behind the last group
+    clean = grads()
+    dy[80] = bad
+    got = grads()
+    others, keep = [0, 2, 3], [i for i in range(212) if i != 80]
+    assert torch.equal(want[0][:70], got[0][:70]) and torch.equal(clean[0][keep], got[0][keep])
+    for i in (1, 2):
+        assert torch.equal(got[i][others], want[i][others]) and not torch.isfinite(got[i][1]).all()
