@@ -120,6 +120,9 @@ def default_status(device) -> torch.Tensor:
     t = _DEFAULT_STATUS.get(idx)
     if t is None:
         t = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", idx))
+        with torch.cuda.device(idx):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()      # once: kernels on other streams report to it next
         _DEFAULT_STATUS[idx] = t
     return t
 
