@@ -134,8 +134,8 @@ def balance_loss(logits: torch.Tensor, topk_idx: torch.Tensor, *, balance_coef: 
     experts masked).  Such tokens get a zero gradient, sequences without any token are left out of the mean, and
     without any token at all the loss is zero.  ``counts`` is [E], or [S, E] with ``seq_rows``, of the copies of tokens that
     take part; it may be changed by the caller.  They are not sizes of groups of packed rows, where the copies of the other
-    tokens may lie too: ``make_plan(topk_idx, E).counts`` are.  The same inputs give the same bits.  Derivatives are reverse mode, of first order.  CPU tensors take plain
-    PyTorch."""
+    tokens may lie too: ``make_plan(topk_idx, E).counts`` are.  The same inputs give the same bits.  Derivatives are reverse
+    mode, of first order.  CPU tensors take plain PyTorch."""
     require(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be [T, E]")
     T, E = logits.shape
     require(topk_idx.dim() == 2 and topk_idx.shape[0] == T and topk_idx.shape[1] >= 1, "topk_idx must be [T, k]")
