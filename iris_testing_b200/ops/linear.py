@@ -206,6 +206,7 @@ def linear(x: torch.Tensor, w_kmajor: torch.Tensor, bias: Optional[torch.Tensor]
     the pre-activation is kept to 16 bits (fp16), or to 11 bits and to 2^-30 (bf16; to 8 bits where 32 neighbouring ones hold
     both a value of 1024 or more and one 2^31 times smaller), and its gradient dz in x's dtype.  fp16 dz are divided by one
     power of two, 2^10 at most, where the call's largest is above 65504, and multiplied with one where it is below 2^-10.
+    A relu's slope is 0 or 1 where its pre-activation is nothing but the sum's rounding.
     Groups that hold more rows than x has, and device-side timeouts, are reported to :func:`check_default_status`; what the
     call returns is then undefined.  The same inputs give the same bits.  Derivatives are reverse mode, of first order.  CPU
     tensors take plain PyTorch."""
