@@ -52,7 +52,7 @@ def reference_under(x, w, b, act, rows, dy, power):
     extra = 2.0 ** -25 * power if top >= 2.0 ** -10 else 2.0 ** -38 * top
     plain = kept.reference(x, w, b, act, rows, dy)
     # what 2^-25 adds to each result there is taken off, and what ``extra`` adds is put on; both without the results' own half step
-    start, out = 0, []
+    start = 0
     (dx, ex), (dw, ew), (db, eb) = plain
     ex, ew = ex.clone(), ew.clone()
     for g, n in enumerate(rows):

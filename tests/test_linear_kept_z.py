@@ -1,6 +1,6 @@
 """The pre-activations that ``linear`` keeps for its backward pass, and gradients held to what they are kept to.
 
-z is kept to 11 bits, off by 2^-11 |z|, and in absolute terms by 2^-30; where 32 neighbouring columns of a row hold both a value of
+z is kept to 11 bits (of fp16 products to 16: see test_linear_fp16_precision.py), off by 2^-11 |z|, and in absolute terms by 2^-30; where 32 neighbouring columns of a row hold both a value of
 1024 or more and one 2^31 times smaller than their largest, to 8 bits, off by 2^-8 |z| whatever the size.  Everything else is bounded
 as in test_linear.py: sums of K products by (K / 16 + 16) 2^-23 of their magnitudes, the activations' slopes by 1.13 and their
 curvatures by 1.2, 32 roundings for computing them, dz and the results rounded to the element type."""
